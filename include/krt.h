@@ -362,6 +362,127 @@ KRT_API size_t krt_paged_attention_prefill_workspace_size(void);
 KRT_API int krt_paged_attention_prefill(const krt_paged_prefill_attention_args* args, void* stream);
 
 /* -------------------------------------------------------------------------
+ * Paged attention with score modifications: the two attentions above for
+ * layers whose scores are capped, biased or masked further.  No counterpart
+ * in the reference.  With p the query's position and s_j = q . k_j:
+ *   x_j = scale * s_j
+ *   x_j = softcap * tanh(x_j / softcap)       softcap > 0
+ *   x_j = x_j - alibi_slopes[h] * |p - j|     alibi_slopes != NULL, fp32 [n_heads]
+ *   key j is visible iff lo <= j < hi:
+ *     lo = max(0, kv_start, window > 0 ? p - window + 1 : 0)
+ *     hi = the sequence's tokens 0 .. p and, in prompts, its prefix
+ *   out = sum_j softmax(x)_j v_j over the visible keys; lse (optional, fp32)
+ *       = log sum_j exp(x_j), natural logarithm
+ * A query that sees nothing gets zeros and lse = -infinity.  Cache values
+ * that are not visible do not enter, NaN and infinities included.  bf16
+ * inputs and output; scores, softmax and sums in fp32, the weights rounded to
+ * bf16 for the product with V.  Pool, block tables, alignment and head_dim as
+ * above; any number of query heads per KV head up to 16; the pool holds
+ * fewer than 2^31 - 16 tokens.  scale 0 = 1 / sqrt(head_dim); scale, softcap and
+ * window must not be negative.  Workspaces are zero-filled once when
+ * allocated; calls that may overlap on the GPU need workspaces of their own.
+ * ---------------------------------------------------------------------- */
+
+/* One query token per sequence, at position p = seq_lens[s] - 1 (its K/V are
+ * already in the pool).  Keys before the window or kv_start are not read. */
+typedef struct krt_paged_attention_mod_args {
+  const void* q;              /* bf16 [num_seqs, q_stride], query head h at h * 128 */
+  const void* kv_pool;
+  const int32_t* block_table; /* [num_seqs, block_table_stride] */
+  const int32_t* seq_lens;    /* [num_seqs]; <= 0: zeros; > max_seq_len: cut there, status bit 8 */
+  void* out;                  /* bf16 [num_seqs, out_stride] */
+  float* lse;                 /* [num_seqs, lse_stride] or NULL */
+  const float* alibi_slopes;  /* [n_heads] or NULL */
+  const int32_t* kv_start;    /* [num_seqs] first visible position, or NULL */
+  int32_t num_seqs, n_heads, n_kv_heads, head_dim;
+  int32_t q_stride, out_stride, lse_stride;
+  int32_t block_table_stride, num_blocks, tokens_per_block;
+  int32_t max_seq_len; /* upper bound of seq_lens: sizes the grid and the workspace */
+  int32_t window;      /* 0 = all, else the last `window` positions, the query's included */
+  float scale, softcap;
+  void* workspace;
+  size_t workspace_bytes;
+} krt_paged_attention_mod_args;
+
+KRT_API size_t krt_paged_attention_mod_workspace_size(int32_t num_seqs, int32_t n_heads, int32_t n_kv_heads,
+                                                      int32_t max_seq_len, int32_t window);
+KRT_API int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args* args, void* stream);
+
+/* Prompt tokens: sequence s has rows q_start[s] .. q_start[s + 1] - 1 of q
+ * and out, at positions q_pos0[s] .., and len_s = q_pos0[s] + its rows tokens
+ * in the pool.  hi = min(len_s, max(p + 1, prefix_lens[s])): the first
+ * prefix_lens[s] tokens are visible to every query of the sequence (also
+ * those before them), the window and kv_start still apply.  kv_start holds
+ * one first position per row (the start of the row's document).  Rows of q
+ * and out beyond q_start[num_seqs] are left as they were.  q_start must not
+ * decrease nor leave 0 .. num_tokens (status bit 8; such parts are left out).
+ * max_kv_len is an upper bound of len_s; a longer sequence is computed all
+ * the same, within its block table (status bit 8 beyond it). */
+typedef struct krt_paged_prefill_attention_mod_args {
+  const void* q;              /* bf16 [num_tokens, q_stride] */
+  const void* kv_pool;
+  const int32_t* block_table; /* [num_seqs, block_table_stride] */
+  const int32_t* q_start;     /* [num_seqs + 1] */
+  const int32_t* q_pos0;      /* [num_seqs], 0 .. 2^30 */
+  void* out;                  /* bf16 [num_tokens, out_stride] */
+  float* lse;                 /* [num_tokens, lse_stride] or NULL */
+  const float* alibi_slopes;  /* [n_heads] or NULL */
+  const int32_t* kv_start;    /* [num_tokens] first visible position of each row, or NULL */
+  const int32_t* prefix_lens; /* [num_seqs] or NULL */
+  int32_t num_tokens, num_seqs, n_heads, n_kv_heads, head_dim;
+  int32_t q_stride, out_stride, lse_stride;
+  int32_t block_table_stride, num_blocks, tokens_per_block;
+  int32_t max_kv_len, window;
+  float scale, softcap;
+  void* workspace;
+  size_t workspace_bytes;
+} krt_paged_prefill_attention_mod_args;
+
+KRT_API size_t krt_paged_attention_prefill_mod_workspace_size(int32_t num_tokens, int32_t num_seqs, int32_t n_heads,
+                                                              int32_t n_kv_heads, int32_t max_kv_len);
+KRT_API int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention_mod_args* args, void* stream);
+
+/* -------------------------------------------------------------------------
+ * Rotary positions of q and k, with k and v appended to the paged cache: the
+ * tail of the fused QKV kernels by itself, for projections that come from
+ * elsewhere and for rotations that those kernels do not have.  No counterpart
+ * in the reference (its RoPE is the half-split rotation of the whole row,
+ * fusion_forge.py:92-110).  Per token t and pair i of the first rotary_dim dims of a q or k head:
+ *   angle = positions[t] * inv_freq[i]
+ *   (a, b) -> (a cos - b sin, b cos + a sin) * factor
+ * with (a, b) = dims (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved;
+ * the other dims pass through.  inv_freq is fp64 and carries any scaling for
+ * long contexts; any int32 position.  k and v go to index cache_index[t]
+ * (NULL: positions[t]) of sequence token_seq[t].  A token with token_seq < 0
+ * is padding: nothing is written for it.  A sequence, index or block outside
+ * the table or pool: q is still written, k and v are not, status bit 8.  Two
+ * tokens of one call must not go to the same slot; q_out must not overlap q,
+ * k or v. */
+typedef struct krt_rope_append_args {
+  const void* q; /* [num_tokens, q_stride] of dtype, head h at h * 128 */
+  const void* k; /* [num_tokens, k_stride] */
+  const void* v; /* [num_tokens, v_stride] */
+  const double* inv_freq;     /* [rotary_dim / 2] */
+  const int32_t* positions;   /* [num_tokens] */
+  const int32_t* cache_index; /* [num_tokens] or NULL */
+  const int32_t* token_seq;   /* [num_tokens] row of block_table, negative: padding */
+  const int32_t* block_table; /* [num_seqs, block_table_stride] */
+  void* kv_pool;
+  void* q_out; /* bf16 [num_tokens, q_out_stride] */
+  int64_t q_stride, k_stride, v_stride, q_out_stride; /* elements; rows 16-byte aligned */
+  int32_t num_tokens, n_heads, n_kv_heads, head_dim, rotary_dim;
+  int32_t interleaved;
+  int32_t dtype; /* of q, k, v: KRT_DTYPE_BFLOAT16 (also 0) or KRT_DTYPE_FLOAT32 */
+  int32_t num_seqs, block_table_stride, num_blocks, tokens_per_block;
+  float factor; /* on cos and sin; 0 = 1 */
+  void* workspace; /* krt_rope_append_workspace_size() bytes, zeroed once: the status word */
+  size_t workspace_bytes;
+} krt_rope_append_args;
+
+KRT_API size_t krt_rope_append_workspace_size(void);
+KRT_API int krt_rope_append(const krt_rope_append_args* args, void* stream);
+
+/* -------------------------------------------------------------------------
  * The rest of a decode step (batch of up to 256 tokens, bf16, fp32
  * accumulation).  The reference has no decoder forward; these are the
  * callers on either side of the hot path that its generation loop

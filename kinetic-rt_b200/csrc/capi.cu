@@ -170,6 +170,18 @@ int make_tmap_bf16_5d_strided(CUtensorMap* map, const void* base, std::initializ
   return KRT_OK;
 }
 
+// The paged pool as boxes of 16 tokens of one KV head, 128-byte swizzled:
+// {64 dims, token (all blocks' tokens in order), dim half, K | V, kv head}.
+// A box is all of the tokens' K and V (four [16 x 128 B] tiles: K lo, K hi,
+// V lo, V hi) or, with `both` false, one of these tiles.
+int make_tmap_pool_kv16(CUtensorMap* map, const void* pool, int num_blocks, int tokens_per_block, int n_kv_heads,
+                        bool both) {
+  const uint64_t token_bytes = (uint64_t)2 * n_kv_heads * kHeadDim * 2;
+  const uint32_t parts = both ? 2 : 1;
+  return make_tmap_bf16_5d_strided(map, pool, {64, (uint64_t)num_blocks * tokens_per_block, 2, 2, (uint64_t)n_kv_heads},
+                                   {token_bytes, 128, (uint64_t)n_kv_heads * 256, 256}, {64, 16, parts, parts, 1});
+}
+
 }  // namespace krt
 
 using namespace krt;

@@ -23,6 +23,8 @@ int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t rows, uint64_
                       uint32_t box_rows, uint32_t kc);
 int make_tmap_bf16_5d_strided(CUtensorMap* map, const void* base, std::initializer_list<uint64_t> dims,
                               std::initializer_list<uint64_t> strides, std::initializer_list<uint32_t> box);
+int make_tmap_pool_kv16(CUtensorMap* map, const void* pool, int num_blocks, int tokens_per_block, int n_kv_heads,
+                        bool both);
 int make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems,
                       uint32_t box_rows);
 

@@ -88,6 +88,45 @@ class PagedPrefillAttentionArgs(ctypes.Structure):
     ]
 
 
+class PagedAttentionModArgs(ctypes.Structure):
+    """krt_paged_attention_mod_args"""
+    _fields_ = [
+        ("q", _vp), ("kv_pool", _vp), ("block_table", _vp), ("seq_lens", _vp), ("out", _vp), ("lse", _vp),
+        ("alibi_slopes", _vp), ("kv_start", _vp),
+        ("num_seqs", _i32), ("n_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
+        ("q_stride", _i32), ("out_stride", _i32), ("lse_stride", _i32),
+        ("block_table_stride", _i32), ("num_blocks", _i32), ("tokens_per_block", _i32),
+        ("max_seq_len", _i32), ("window", _i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagedPrefillAttentionModArgs(ctypes.Structure):
+    """krt_paged_prefill_attention_mod_args"""
+    _fields_ = [
+        ("q", _vp), ("kv_pool", _vp), ("block_table", _vp), ("q_start", _vp), ("q_pos0", _vp), ("out", _vp),
+        ("lse", _vp), ("alibi_slopes", _vp), ("kv_start", _vp), ("prefix_lens", _vp),
+        ("num_tokens", _i32), ("num_seqs", _i32), ("n_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
+        ("q_stride", _i32), ("out_stride", _i32), ("lse_stride", _i32),
+        ("block_table_stride", _i32), ("num_blocks", _i32), ("tokens_per_block", _i32),
+        ("max_kv_len", _i32), ("window", _i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class RopeAppendArgs(ctypes.Structure):
+    """krt_rope_append_args"""
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("inv_freq", _vp), ("positions", _vp), ("cache_index", _vp),
+        ("token_seq", _vp), ("block_table", _vp), ("kv_pool", _vp), ("q_out", _vp),
+        ("q_stride", _i64), ("k_stride", _i64), ("v_stride", _i64), ("q_out_stride", _i64),
+        ("num_tokens", _i32), ("n_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32), ("rotary_dim", _i32),
+        ("interleaved", _i32), ("dtype", _i32),
+        ("num_seqs", _i32), ("block_table_stride", _i32), ("num_blocks", _i32), ("tokens_per_block", _i32),
+        ("factor", ctypes.c_float), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class GateUpArgs(ctypes.Structure):
     """krt_gate_up_args"""
     _fields_ = [
@@ -144,6 +183,12 @@ SIGNATURES = {
     "krt_paged_attention_decode": (ctypes.c_int, [ctypes.POINTER(PagedAttentionArgs), _vp]),
     "krt_paged_attention_prefill_workspace_size": (ctypes.c_size_t, []),
     "krt_paged_attention_prefill": (ctypes.c_int, [ctypes.POINTER(PagedPrefillAttentionArgs), _vp]),
+    "krt_paged_attention_mod_workspace_size": (ctypes.c_size_t, [_i32, _i32, _i32, _i32, _i32]),
+    "krt_paged_attention_decode_mod": (ctypes.c_int, [ctypes.POINTER(PagedAttentionModArgs), _vp]),
+    "krt_paged_attention_prefill_mod_workspace_size": (ctypes.c_size_t, [_i32, _i32, _i32, _i32, _i32]),
+    "krt_paged_attention_prefill_mod": (ctypes.c_int, [ctypes.POINTER(PagedPrefillAttentionModArgs), _vp]),
+    "krt_rope_append_workspace_size": (ctypes.c_size_t, []),
+    "krt_rope_append": (ctypes.c_int, [ctypes.POINTER(RopeAppendArgs), _vp]),
     "krt_projection_workspace_size": (ctypes.c_size_t, [_i32, _i32]),
     "krt_gate_up_swiglu": (ctypes.c_int, [ctypes.POINTER(GateUpArgs), _vp]),
     "krt_lm_head_argmax": (ctypes.c_int, [ctypes.POINTER(LmHeadArgs), _vp]),
@@ -386,6 +431,205 @@ def prefill_attention_args(q, kv_pool, block_table, q_start, q_pos0, out, n_head
 
 def paged_attention_prefill(args, stream=None):
     check(lib().krt_paged_attention_prefill(ctypes.byref(args), _stream(stream)))
+
+
+# ------------------------- attention with score modifications, rotary append
+def _check_cuda(who, dtype=None, **tensors):
+    """Tensors (None: not given) on one CUDA device, of `dtype`, elements of a
+    row adjacent; returns the device."""
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{who}: {name} must be on a CUDA device, found {t.device}")
+        if device is not None and t.device != device:
+            raise ValueError(f"{who}: {name} is on {t.device}, other arguments on {device}")
+        device = t.device
+        if dtype is not None and t.dtype != dtype:
+            raise ValueError(f"{who}: {name} must be {dtype}, found {t.dtype}")
+        if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{who}: {name}'s last dimension must be contiguous")
+    return device
+
+
+def _check_shape(who, name, t, *shape):
+    """t has at least `shape` (None: any) elements per dimension; None passes."""
+    if t is None:
+        return
+    if t.dim() != len(shape) or any(w is not None and n < w for n, w in zip(t.shape, shape)):
+        raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, at least {shape} is needed")
+
+
+def _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_heads):
+    import torch
+    _check_cuda(who, torch.int32, block_table=block_table)
+    if block_table.dim() != 2:
+        raise ValueError(f"{who}: block_table must be [num_seqs, blocks]")
+    _check_cuda(who, torch.bfloat16, kv_pool=kv_pool)
+    if not kv_pool.is_contiguous() or kv_pool.numel() < num_blocks * tokens_per_block * 2 * n_kv_heads * 128:
+        raise ValueError(f"{who}: kv_pool must be contiguous and hold num_blocks blocks")
+
+
+def _check_current(who, args):
+    """Launches go to the current device's current stream: the tensors live there."""
+    import torch
+    if args._device.index != torch.cuda.current_device():
+        raise ValueError(f"{who}: the tensors are on {args._device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()} (torch.cuda.set_device)")
+
+
+def attention_mod_workspace_bytes(num_seqs, n_heads, n_kv_heads, max_seq_len, window=0):
+    return int(lib().krt_paged_attention_mod_workspace_size(num_seqs, n_heads, n_kv_heads, max_seq_len, window))
+
+
+def attention_mod_args(q, kv_pool, block_table, seq_lens, out, n_heads, n_kv_heads, num_blocks, tokens_per_block,
+                       max_seq_len, workspace, scale=0.0, softcap=0.0, window=0, alibi_slopes=None, kv_start=None,
+                       lse=None, head_dim=128):
+    """Decode attention with score modifications.  q / out: bf16 [num_seqs, >=
+    n_heads * 128]; alibi_slopes fp32 [n_heads]; kv_start int32 [num_seqs];
+    lse fp32 [num_seqs, >= n_heads] out."""
+    import torch
+    who = "paged_attention_decode_mod"
+    device = _check_cuda(who, q=q, kv_pool=kv_pool, block_table=block_table, seq_lens=seq_lens, out=out,
+                         alibi_slopes=alibi_slopes, kv_start=kv_start, lse=lse, workspace=workspace)
+    S, H = int(q.shape[0]), int(n_heads)
+    _check_cuda(who, torch.bfloat16, q=q, out=out)
+    _check_cuda(who, torch.float32, alibi_slopes=alibi_slopes, lse=lse)
+    _check_cuda(who, torch.int32, seq_lens=seq_lens, kv_start=kv_start)
+    _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_heads)
+    _check_shape(who, "q", q, None, H * head_dim)
+    _check_shape(who, "out", out, S, H * head_dim)
+    _check_shape(who, "block_table", block_table, S, None)
+    _check_shape(who, "seq_lens", seq_lens, S)
+    _check_shape(who, "kv_start", kv_start, S)
+    _check_shape(who, "alibi_slopes", alibi_slopes, H)
+    _check_shape(who, "lse", lse, S, H)
+    a = PagedAttentionModArgs()
+    a.q, a.kv_pool, a.block_table, a.seq_lens, a.out = (_ptr(q), _ptr(kv_pool), _ptr(block_table), _ptr(seq_lens),
+                                                        _ptr(out))
+    a.lse, a.alibi_slopes, a.kv_start = _ptr(lse), _ptr(alibi_slopes), _ptr(kv_start)
+    a.num_seqs, a.n_heads, a.n_kv_heads, a.head_dim = S, H, int(n_kv_heads), int(head_dim)
+    a.q_stride, a.out_stride = int(q.stride(0)), int(out.stride(0))
+    a.lse_stride = 0 if lse is None else int(lse.stride(0))
+    a.block_table_stride, a.num_blocks = int(block_table.stride(0)), int(num_blocks)
+    a.tokens_per_block, a.max_seq_len, a.window = int(tokens_per_block), int(max_seq_len), int(window)
+    a.scale, a.softcap = float(scale), float(softcap)
+    a.workspace = _ptr(workspace)
+    a.workspace_bytes = workspace.numel() * workspace.element_size()
+    a._refs = (q, kv_pool, block_table, seq_lens, out, lse, alibi_slopes, kv_start, workspace)
+    a._device = device
+    return a
+
+
+def paged_attention_decode_mod(args, stream=None):
+    _check_current("paged_attention_decode_mod", args)
+    check(lib().krt_paged_attention_decode_mod(ctypes.byref(args), _stream(stream)))
+
+
+def prefill_attention_mod_workspace_bytes(num_tokens, num_seqs, n_heads, n_kv_heads, max_kv_len):
+    return int(lib().krt_paged_attention_prefill_mod_workspace_size(num_tokens, num_seqs, n_heads, n_kv_heads,
+                                                                    max_kv_len))
+
+
+def prefill_attention_mod_args(q, kv_pool, block_table, q_start, q_pos0, out, n_heads, n_kv_heads, num_blocks,
+                               tokens_per_block, max_kv_len, workspace, scale=0.0, softcap=0.0, window=0,
+                               alibi_slopes=None, kv_start=None, prefix_lens=None, lse=None, head_dim=128):
+    """Prompt attention with score modifications.  q / out: bf16 [T, >= n_heads *
+    128] (sequence s's query rows q_start[s] .. q_start[s + 1] - 1); q_start
+    int32 [num_seqs + 1]; q_pos0, prefix_lens int32 [num_seqs]; kv_start int32
+    [T]; alibi_slopes fp32 [n_heads]; lse fp32 [T, >= n_heads] out."""
+    import torch
+    who = "paged_attention_prefill_mod"
+    device = _check_cuda(who, q=q, kv_pool=kv_pool, block_table=block_table, q_start=q_start, q_pos0=q_pos0, out=out,
+                         alibi_slopes=alibi_slopes, kv_start=kv_start, prefix_lens=prefix_lens, lse=lse,
+                         workspace=workspace)
+    T, S, H = int(q.shape[0]), int(q_pos0.shape[0]), int(n_heads)
+    _check_cuda(who, torch.bfloat16, q=q, out=out)
+    _check_cuda(who, torch.float32, alibi_slopes=alibi_slopes, lse=lse)
+    _check_cuda(who, torch.int32, q_start=q_start, q_pos0=q_pos0, kv_start=kv_start, prefix_lens=prefix_lens)
+    _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_heads)
+    _check_shape(who, "q", q, None, H * head_dim)
+    _check_shape(who, "out", out, T, H * head_dim)
+    _check_shape(who, "q_start", q_start, S + 1)
+    _check_shape(who, "block_table", block_table, S, None)
+    _check_shape(who, "kv_start", kv_start, T)
+    _check_shape(who, "prefix_lens", prefix_lens, S)
+    _check_shape(who, "alibi_slopes", alibi_slopes, H)
+    _check_shape(who, "lse", lse, T, H)
+    a = PagedPrefillAttentionModArgs()
+    a.q, a.out, a.kv_pool, a.block_table = _ptr(q), _ptr(out), _ptr(kv_pool), _ptr(block_table)
+    a.q_start, a.q_pos0, a.lse, a.alibi_slopes = _ptr(q_start), _ptr(q_pos0), _ptr(lse), _ptr(alibi_slopes)
+    a.kv_start, a.prefix_lens = _ptr(kv_start), _ptr(prefix_lens)
+    a.num_tokens, a.num_seqs, a.n_heads, a.n_kv_heads, a.head_dim = T, S, H, int(n_kv_heads), int(head_dim)
+    a.q_stride, a.out_stride = int(q.stride(0)), int(out.stride(0))
+    a.lse_stride = 0 if lse is None else int(lse.stride(0))
+    a.block_table_stride, a.num_blocks = int(block_table.stride(0)), int(num_blocks)
+    a.tokens_per_block, a.max_kv_len, a.window = int(tokens_per_block), int(max_kv_len), int(window)
+    a.scale, a.softcap = float(scale), float(softcap)
+    a.workspace = _ptr(workspace)
+    a.workspace_bytes = workspace.numel() * workspace.element_size()
+    a._refs = (q, kv_pool, block_table, q_start, q_pos0, out, lse, alibi_slopes, kv_start, prefix_lens, workspace)
+    a._device = device
+    return a
+
+
+def paged_attention_prefill_mod(args, stream=None):
+    _check_current("paged_attention_prefill_mod", args)
+    check(lib().krt_paged_attention_prefill_mod(ctypes.byref(args), _stream(stream)))
+
+
+def rope_append_workspace_bytes():
+    return int(lib().krt_rope_append_workspace_size())
+
+
+def rope_append_args(q, k, v, inv_freq, positions, token_seq, block_table, kv_pool, q_out, n_heads, n_kv_heads,
+                     num_blocks, tokens_per_block, workspace, interleaved=False, factor=1.0, cache_index=None,
+                     head_dim=128):
+    """q [T, n_heads * 128], k and v [T, n_kv_heads * 128]: all bf16 or all fp32,
+    rows of any stride (views of one fused projection); inv_freq fp64
+    [rotary_dim / 2]; q_out bf16 [T, >= n_heads * 128]; positions, token_seq,
+    cache_index int32 [T]."""
+    import torch
+    who = "rope_append"
+    device = _check_cuda(who, q=q, k=k, v=v, inv_freq=inv_freq, positions=positions, token_seq=token_seq,
+                         block_table=block_table, kv_pool=kv_pool, q_out=q_out, cache_index=cache_index,
+                         workspace=workspace)
+    T, H, K = int(q.shape[0]), int(n_heads), int(n_kv_heads)
+    _check_cuda(who, q.dtype, q=q, k=k, v=v)
+    _check_cuda(who, torch.bfloat16, q_out=q_out)
+    _check_cuda(who, torch.float64, inv_freq=inv_freq)
+    _check_cuda(who, torch.int32, positions=positions, token_seq=token_seq, cache_index=cache_index)
+    _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_heads)
+    _check_shape(who, "q", q, None, H * head_dim)
+    _check_shape(who, "k", k, T, K * head_dim)
+    _check_shape(who, "v", v, T, K * head_dim)
+    _check_shape(who, "q_out", q_out, T, H * head_dim)
+    for name, t in (("positions", positions), ("token_seq", token_seq), ("cache_index", cache_index)):
+        _check_shape(who, name, t, T)
+    _check_shape(who, "inv_freq", inv_freq, 1)
+    if factor == 0.0:
+        raise ValueError(f"{who}: factor must not be 0")
+    a = RopeAppendArgs()
+    a.q, a.k, a.v, a.inv_freq, a.positions = _ptr(q), _ptr(k), _ptr(v), _ptr(inv_freq), _ptr(positions)
+    a.cache_index, a.token_seq, a.block_table = _ptr(cache_index), _ptr(token_seq), _ptr(block_table)
+    a.kv_pool, a.q_out = _ptr(kv_pool), _ptr(q_out)
+    a.q_stride, a.k_stride, a.v_stride = int(q.stride(0)), int(k.stride(0)), int(v.stride(0))
+    a.q_out_stride = int(q_out.stride(0))
+    a.num_tokens, a.n_heads, a.n_kv_heads, a.head_dim = T, H, K, int(head_dim)
+    a.rotary_dim, a.interleaved, a.dtype = 2 * int(inv_freq.shape[0]), int(bool(interleaved)), _dtype_code(q)
+    a.num_seqs, a.block_table_stride = int(block_table.shape[0]), int(block_table.stride(0))
+    a.num_blocks, a.tokens_per_block, a.factor = int(num_blocks), int(tokens_per_block), float(factor)
+    a.workspace = _ptr(workspace)
+    a.workspace_bytes = workspace.numel() * workspace.element_size()
+    a._refs = (q, k, v, inv_freq, positions, cache_index, token_seq, block_table, kv_pool, q_out, workspace)
+    a._device = device
+    return a
+
+
+def rope_append(args, stream=None):
+    _check_current("rope_append", args)
+    check(lib().krt_rope_append(ctypes.byref(args), _stream(stream)))
 
 
 # ------------------------------------------------- rest of the decode step

@@ -56,6 +56,18 @@ def rope_cache(torch, max_position, head_dim, theta, device="cuda"):
     return emb.cos().float().to(device), emb.sin().float().to(device)
 
 
+def rope_inv_freq(torch, rotary_dim, theta, stretch=1.0, trained_context=8192, device="cuda"):
+    """Rotary frequencies of rope_append (fp64 [rotary_dim / 2]) and the factor
+    on cos and sin that goes with them.  stretch > 1 scales for long contexts:
+    a frequency that makes fewer than one turn in `trained_context` tokens is
+    divided by `stretch`, one that makes more than four is kept, those between
+    are blended; the factor is 0.1 ln(stretch) + 1."""
+    import math
+    f = float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    keep = ((trained_context * f / (2 * math.pi) - 1) / 3).clamp(0, 1)
+    return (f * keep + f / stretch * (1 - keep)).to(device), 0.1 * math.log(stretch) + 1
+
+
 def vocab_shard(vocab, rank, world):
     """Rows [lo, hi) of the vocabulary on `rank` (torch.chunk along rows)."""
     step = -(-vocab // world)
