@@ -17,6 +17,9 @@ struct ScoreMod {
   float cap_in;      // 2 * log2(e) * scale / cap: ex2(s * cap_in) = e^(2 x / c)
   const float* slopes;  // [n_heads] or NULL
   int window;        // 0 = none
+  // cap by polynomial while |s| <= poly_max: x = s * P(s^2), see cap_poly
+  float poly[5];
+  float poly_max;    // negative: never
 };
 
 inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, int window) {
@@ -28,6 +31,19 @@ inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, 
   m.cap_in = softcap > 0.f ? 2.f * kLog2e * sc / softcap : 0.f;
   m.slopes = slopes;
   m.window = window;
+  // cap2 * tanh(u), u = a s, as an odd polynomial in s (cap_poly's coefficients times cap2 a^(2k+1));
+  // left out where powers of a could leave the range of a float
+  m.poly_max = -1.f;
+  if (softcap > 0.f) {
+    static const double c[5] = {0.9999985098838806, -0.33326974511146545, 0.13257454335689545, -0.05019525811076164,
+                                0.013194185681641102};
+    const double a = (double)sc / softcap;
+    if (a > 1e-4 && a < 1e3 && softcap < 1e6f) {
+      double f = a * m.cap2;
+      for (int k = 0; k < 5; ++k, f *= a * a) m.poly[k] = (float)(c[k] * f);
+      m.poly_max = (float)(0.7 / a);
+    }
+  }
   return m;
 }
 
@@ -52,6 +68,47 @@ __device__ __forceinline__ float rcp_approx(float x) {
 __device__ __forceinline__ float cap_score(float s, float cap_in, float cap2) {
   const float e = ex2(s * cap_in);
   return fmaf(-2.f * cap2, rcp_approx(1.f + e), cap2);
+}
+
+// ---- two floats in one 64-bit register: one issue slot for two multiply-adds
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// P(w), w = s^2, of cap2 * tanh(scale s / c) = s * P(s^2) for |u| = |scale s /
+// c| <= 0.7: the degree-4 polynomial in u^2 with the smallest largest error of
+// u * P(u^2) against tanh(u) there (fitted by reweighted least squares), off
+// by at most 9.5e-8.  Scores beyond that take cap_score.  Five multiply-adds
+// and no special-function operation, of which the softmax needs all: tanh by
+// ex2 and rcp would triple them.
+__device__ __forceinline__ f32x2 cap_poly(f32x2 w, const f32x2* c) {
+  return fma2(fma2(fma2(fma2(c[4], w, c[3]), w, c[2]), w, c[1]), w, c[0]);
 }
 
 }  // namespace krt

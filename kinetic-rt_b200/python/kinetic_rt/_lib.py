@@ -471,12 +471,27 @@ def _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_h
         raise ValueError(f"{who}: kv_pool must be contiguous and hold num_blocks blocks")
 
 
-def _check_current(who, args):
-    """Launches go to the current device's current stream: the tensors live there."""
+def _launch(who, fn, args, stream):
+    """Launches go to the current device's current stream: the tensors live
+    there.  A decode loop pays for every call, so the struct's byref and its
+    device index are kept with it and the stream is read as a raw handle."""
     import torch
-    if args._device.index != torch.cuda.current_device():
-        raise ValueError(f"{who}: the tensors are on {args._device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()} (torch.cuda.set_device)")
+    if stream is None:
+        device = torch._C._cuda_getDevice()
+        if device != args._index:
+            raise ValueError(f"{who}: the tensors are on cuda:{args._index}, the current device is cuda:{device} "
+                             "(torch.cuda.set_device)")
+        stream = torch._C._cuda_getCurrentRawStream(device)
+    rc = fn(args._ref, stream)
+    if rc != KRT_OK:
+        check(rc)
+
+
+def _keep(args, device, *refs):
+    args._refs = refs
+    args._index = device.index
+    args._ref = ctypes.byref(args)
+    return args
 
 
 def attention_mod_workspace_bytes(num_seqs, n_heads, n_kv_heads, max_seq_len, window=0):
@@ -517,14 +532,11 @@ def attention_mod_args(q, kv_pool, block_table, seq_lens, out, n_heads, n_kv_hea
     a.scale, a.softcap = float(scale), float(softcap)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()
-    a._refs = (q, kv_pool, block_table, seq_lens, out, lse, alibi_slopes, kv_start, workspace)
-    a._device = device
-    return a
+    return _keep(a, device, q, kv_pool, block_table, seq_lens, out, lse, alibi_slopes, kv_start, workspace)
 
 
 def paged_attention_decode_mod(args, stream=None):
-    _check_current("paged_attention_decode_mod", args)
-    check(lib().krt_paged_attention_decode_mod(ctypes.byref(args), _stream(stream)))
+    _launch("paged_attention_decode_mod", lib().krt_paged_attention_decode_mod, args, stream)
 
 
 def prefill_attention_mod_workspace_bytes(num_tokens, num_seqs, n_heads, n_kv_heads, max_kv_len):
@@ -569,14 +581,11 @@ def prefill_attention_mod_args(q, kv_pool, block_table, q_start, q_pos0, out, n_
     a.scale, a.softcap = float(scale), float(softcap)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()
-    a._refs = (q, kv_pool, block_table, q_start, q_pos0, out, lse, alibi_slopes, kv_start, prefix_lens, workspace)
-    a._device = device
-    return a
+    return _keep(a, device, q, kv_pool, block_table, q_start, q_pos0, out, lse, alibi_slopes, kv_start, prefix_lens, workspace)
 
 
 def paged_attention_prefill_mod(args, stream=None):
-    _check_current("paged_attention_prefill_mod", args)
-    check(lib().krt_paged_attention_prefill_mod(ctypes.byref(args), _stream(stream)))
+    _launch("paged_attention_prefill_mod", lib().krt_paged_attention_prefill_mod, args, stream)
 
 
 def rope_append_workspace_bytes():
@@ -622,14 +631,11 @@ def rope_append_args(q, k, v, inv_freq, positions, token_seq, block_table, kv_po
     a.num_blocks, a.tokens_per_block, a.factor = int(num_blocks), int(tokens_per_block), float(factor)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()
-    a._refs = (q, k, v, inv_freq, positions, cache_index, token_seq, block_table, kv_pool, q_out, workspace)
-    a._device = device
-    return a
+    return _keep(a, device, q, k, v, inv_freq, positions, cache_index, token_seq, block_table, kv_pool, q_out, workspace)
 
 
 def rope_append(args, stream=None):
-    _check_current("rope_append", args)
-    check(lib().krt_rope_append(ctypes.byref(args), _stream(stream)))
+    _launch("rope_append", lib().krt_rope_append, args, stream)
 
 
 # ------------------------------------------------- rest of the decode step
