@@ -9,35 +9,35 @@
 //
 // One CTA works on 256 rows = two tiles of 128 rows; a tile holds 128 / G
 // query tokens x the G query heads of one KV head (rows token-major), so a
-// K/V block that is fetched serves all of them.  Twenty warps:
-//   * warps 0-7 and 8-15: softmax of tile 0 and tile 1.  Two threads share a
-//     row (a TMEM lane): of a block's 128 keys the first takes 0-31 and 64-95,
-//     the second the others;
-//   * warp 16: TMA producer.  K and V blocks of 128 tokens alternate in a ring
-//     of five 32 KB stages; a block is eight 16-token pages, two boxes each;
-//   * warp 17: issues the UMMAs: S = Q K^T (M = N = 128, both operands in
-//     shared memory) and O += P V (P from TMEM, V as the MN-major operand);
-//   * warps 18 and 19 only complete the warpgroup that gives up registers.
-// TMEM: S0, S1, O0, O1, 128 columns each (all 512).  P (bf16, 64 columns)
-// overwrites its S.  Issue order QK0 QK1 | PV0 QK0' PV1 QK1' ...: while the
-// softmax of one tile runs, the tensor core works for the other, and P V of
-// the first 64 keys starts while the weights of the others are computed.
+// K/V block that is fetched serves all of them.  Twelve warps:
+//   * warps 0-3 and 4-7: softmax of tile 0 and tile 1, one thread per row (TMEM
+//     lane), so maxima and sums need no exchange;
+//   * warps 8 and 11: TMA producers of K and of V.  Blocks of 64 tokens, 16 KB
+//     each, in two rings of five stages; a block is four 16-token pages, two
+//     boxes each;
+//   * warps 9 and 10: issue the UMMAs of tile 0 and tile 1: S = Q K^T (M = 128,
+//     N = 64, both operands in shared memory) and O += P V (P from TMEM, V as
+//     the MN-major operand).  Two warps, because the waits, descriptors and
+//     commits of a step take longer than its 12 MMAs (one warp for both tiles:
+//     2600 cycles a step, of which the tensor core worked half).
+// TMEM, per tile: two S buffers of 64 columns and O of 128 (all 512 columns).
+// P (bf16, 32 columns) overwrites its S.  Each tile has two blocks in flight:
+// while the softmax works on block g, the tensor core has P V of block g - 1
+// and Q K^T of block g + 1 of the same tile to do, and those of the other
+// tile.  With one buffer of 128 columns per tile the chain S -> weights -> P V
+// -> next S bounded the kernel (4150 cycles for 128 keys and both tiles, where
+// tensor core and special-function units need 2048 each).
 //
-// What bounds it: per block and pair of tiles the tensor core needs 2048
-// cycles, and so do the 2 x 128 x 128 ex2 of the special-function units (one a
-// score, 16 a cycle); a tile's chain S -> weights -> P V -> next S must fit
-// into the same time.  Hence no step that can be spared lies in the chain:
+// What bounds it now: per 128 keys and pair of tiles the tensor core needs
+// about 2560 cycles (2048 of arithmetic; at N = 64 Q K^T reads 6 KB of shared
+// memory per 32 cycles of it), the special-function units 2048 for one ex2 a
+// score.  Steps that are spared:
 //   * the reference that scores are taken against is the row's old maximum
 //     unless it grew by more than 2^8 (weights then stay below 256, and bf16
-//     and the fp32 sum lose nothing by it).  The two threads of a row only
-//     agree, by one barrier that ors their votes, that nothing grew; where it
-//     did they exchange maxima and rescale O and the sum.  MMAs of the issuing
-//     thread run in order, so a full S says that the tile's previous P V is
-//     done and O may be rescaled;
+//     and the fp32 sum lose nothing by it); only then O and the sum are
+//     rescaled, after the tile's last P V;
 //   * the cap is a polynomial of the score while scores are well below it, and
-//     its value at the row's largest |score| serves as the reference;
-//   * a quarter of the weights without a cap take 2^x by polynomial on the
-//     multiply-add pipe.
+//     its value at the row's largest |score| serves as the reference.
 //
 // Statistics, sums and O are fp32; P is rounded to bf16 for P V (2^-9 of each
 // weight, as V is).
@@ -62,13 +62,15 @@
 namespace krt {
 
 constexpr int kApmRows = 128;    // rows of a tile (TMEM lanes)
-constexpr int kApmBlock = 128;   // keys per block
+constexpr int kApmBlock = 64;    // keys per block
 constexpr int kApmPage = 16;     // tokens per TMA box
-constexpr int kApmStages = 5;
-constexpr int kApmSoftmaxWarps = 16;
-constexpr int kApmThreads = 640;
-constexpr uint32_t kApmTileBytes = 32768;  // 128 rows x 128 dims bf16, two [128 x 128 B] halves
+constexpr int kApmStages = 5;    // of K, and of V
+constexpr int kApmSoftmaxWarps = 8;
+constexpr int kApmThreads = 384;
+constexpr uint32_t kApmTileBytes = 32768;  // Q tile: 128 rows x 128 dims bf16, two [128 x 128 B] halves
 constexpr uint32_t kApmHalf = 16384;
+constexpr uint32_t kApmKvBytes = 16384;    // K or V block: 64 tokens x 128 dims, two [64 x 128 B] halves
+constexpr uint32_t kApmKvHalf = 8192;
 constexpr float kApmLazy = 8.f;   // growth of a row's maximum (base 2) that is left unscaled
 constexpr float kApmBound = 50.f; // largest reference (base 2) that may lie above the row's maximum
 constexpr int kApmMaxPos = 1 << 30;
@@ -90,39 +92,40 @@ struct ApmParams {
 };
 
 struct ApmSmemTail {
-  uint64_t full[kApmStages];
-  uint64_t empty[kApmStages];
+  uint64_t full[2][kApmStages];   // K, V
+  uint64_t empty[2][kApmStages];
   uint64_t q_full;
-  uint64_t s_full[2];
-  uint64_t p_full[2][2];  // per tile: P of keys 0-63, of keys 64-127
-  uint64_t o_full[2];
-  uint64_t drain;      // the MMAs issued before an abort
+  uint64_t s_full[2][2];  // per tile and buffer
+  uint64_t p_full[2][2];
+  uint64_t o_done[2];     // per tile: one phase per P V
+  uint64_t o_last[2];     // per tile: the last P V (two may be under way when the last P is reported)
+  uint64_t drain[2];      // per tile: the MMAs issued before an abort
   uint32_t tmem_base;
-  int issued;          // K/V stages requested
+  int issued[2];          // blocks of K and V requested
   int abort;
-  int poison;          // a V value that is not finite was taken out of a partly visible block
-  // this CTA's work, read from here where it is needed: registers are short,
-  // and a spilled one costs an L2 round trip (640 stacks do not fit in L1)
-  int seq, tile;
-  int t_first, q_len, tok0, pos0;  // first row and rows of the sequence, first token of the tiles, its position
-  int lo_min, lo_max, hi_min, hi_max;  // over the CTA's live rows
+  int poison;             // a V value that is not finite was taken out of a partly visible block
+  int seq, tile;          // this CTA's work
+  int t_first, q_len, tok0, pos0;  // first row and rows of the sequence, first token of the tiles, position of token 0
+  int lo_min[2], hi_max[2];        // per tile, over its live rows
+  int lo_max, hi_min;              // over the CTA's live rows
   int scan[kApmThreads / 32];
-  uint32_t bad[8];     // per block (ring): pages that could not be looked up
-  float row_x[2][2][kApmRows];  // exchanged between the two threads of a row
+  uint32_t bad[16];       // per block (ring): pages that could not be looked up
 };
 
 // (no room to round the base up: the kernel checks that it is 1024-byte aligned)
-inline size_t apm_smem_bytes() { return (size_t)(2 + kApmStages) * kApmTileBytes + sizeof(ApmSmemTail); }
+inline size_t apm_smem_bytes() {
+  return (size_t)2 * kApmTileBytes + (size_t)2 * kApmStages * kApmKvBytes + sizeof(ApmSmemTail);
+}
 
 __device__ __forceinline__ void apm_fail(const ApmParams& p, ApmSmemTail* tl, int code) {
   atomicOr(p.status, code);
   *reinterpret_cast<volatile int*>(&tl->abort) = 1;
 }
 
-// Register split after the prologue: 640 threads start with 96 registers each
-// (61440); 512 x 104 + 128 x 64 = 61440.
-constexpr int kApmRegsSoftmax = 104;
-constexpr int kApmRegsOther = 64;
+// Register split after the prologue: 384 threads start with 168 registers each
+// (64512); 256 x 216 + 128 x 72 = 64512.
+constexpr int kApmRegsSoftmax = 216;
+constexpr int kApmRegsOther = 72;
 template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -134,31 +137,6 @@ __device__ __forceinline__ void regs_dec() {
 
 // Exponent bits all ones in either bf16 half of w: a 1 in bit 15 or 31.
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
-
-// 2^y of two values by polynomial: y = n + f, |f| <= 1/2 (n by adding 1.5 2^23,
-// whose low mantissa bits then hold n), 2^f by the degree-4 polynomial with the
-// smallest largest relative error (2.6e-6, fitted by reweighted least squares),
-// n added to the exponent.  y is raised to -126: weights below 2^-126 of the
-// reference come out as that, not 0, -inf included, so masked scores must not
-// come here; NaN stays NaN.
-__device__ __forceinline__ void ex2_poly2(f32x2 y, float& e0, float& e1) {
-  float y0, y1, t0, t1;
-  unpack2(y, y0, y1);
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y0) : "f"(y0), "f"(-126.f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y1) : "f"(y1), "f"(-126.f));
-  y = pack2(y0, y1);
-  constexpr float kMagic = 12582912.f;
-  const f32x2 t = add2(y, pack2(kMagic, kMagic));
-  const f32x2 f = add2(y, mul2(add2(t, pack2(-kMagic, -kMagic)), pack2(-1.f, -1.f)));
-  f32x2 q = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f, pack2(0.05591786280274391f, 0.05591786280274391f));
-  q = fma2(q, f, pack2(0.240247443318367f, 0.240247443318367f));
-  q = fma2(q, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-  q = fma2(q, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-  unpack2(q, e0, e1);
-  unpack2(t, t0, t1);
-  e0 = __uint_as_float(__float_as_uint(e0) + (__float_as_uint(t0) << 23));
-  e1 = __uint_as_float(__float_as_uint(e1) + (__float_as_uint(t1) << 23));
-}
 
 // Pool slot of position j of the sequence, or -1.
 __device__ __forceinline__ long long apm_slot(const ApmParams& p, const int32_t* table, int j) {
@@ -179,37 +157,40 @@ __global__ void __launch_bounds__(kApmThreads, 1)
     return;
   }
   uint8_t* q_smem = smem;
-  uint8_t* kv_smem = smem + 2 * kApmTileBytes;
-  ApmSmemTail* tl = reinterpret_cast<ApmSmemTail*>(smem + (size_t)(2 + kApmStages) * kApmTileBytes);
+  uint8_t* k_smem = smem + 2 * kApmTileBytes;
+  uint8_t* v_smem = k_smem + kApmStages * kApmKvBytes;
+  ApmSmemTail* tl = reinterpret_cast<ApmSmemTail*>(v_smem + kApmStages * kApmKvBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.group, tt = p.tile_tokens;
 
   if (tid == 0) {
-    for (int s = 0; s < kApmStages; ++s) {
-      mbar_init(&tl->full[s], 1);
-      mbar_init(&tl->empty[s], 1);
+    for (int i = 0; i < 2; ++i) {
+      for (int s = 0; s < kApmStages; ++s) {
+        mbar_init(&tl->full[i][s], 1);
+        mbar_init(&tl->empty[i][s], 2);  // both tiles' MMAs
+      }
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&tl->s_full[i][s], 1);
+        mbar_init(&tl->p_full[i][s], 4);
+      }
+      mbar_init(&tl->o_done[i], 1);
+      mbar_init(&tl->o_last[i], 1);
+      mbar_init(&tl->drain[i], 1);
+      tl->issued[i] = 0;
+      tl->lo_min[i] = INT_MAX;
+      tl->hi_max[i] = 0;
     }
     mbar_init(&tl->q_full, 1);
-    mbar_init(&tl->drain, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&tl->s_full[i], 1);
-      mbar_init(&tl->p_full[i][0], 8);
-      mbar_init(&tl->p_full[i][1], 8);
-      mbar_init(&tl->o_full[i], 1);
-    }
     fence_mbar_init();
     tl->abort = 0;
-    tl->issued = 0;
     tl->poison = 0;
     tl->seq = -1;
-    tl->lo_min = INT_MAX;
     tl->lo_max = 0;
     tl->hi_min = INT_MAX;
-    tl->hi_max = 0;
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_kv);
   }
-  if (warp == 17) {
+  if (warp == 9) {
     tmem_alloc(&tl->tmem_base, 512);
     tmem_relinquish();
   }
@@ -283,7 +264,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       tl->pos0 = pos0;
       if (!pos_ok) atomicOr(p.status, kStatusBadBlock);
     }
-    const int r = tid & 127, tok = tok0 + (warp >> 3) * tt + r / G;
+    const int r = tid & 127, tok = tok0 + (warp >> 2) * tt + r / G;
     valid = seq >= 0 && warp < kApmSoftmaxWarps && r < tt * G && tok < q_len;
     if (valid && pos_ok) {
       const int pos = pos0 + tok;
@@ -304,182 +285,170 @@ __global__ void __launch_bounds__(kApmThreads, 1)
     if (warp < kApmSoftmaxWarps && lane == 0) {
       atomicMax(&tl->lo_max, w_lo);
       atomicMin(&tl->hi_min, w_hi);
-      atomicMin(&tl->lo_min, w_lo_min);
-      atomicMax(&tl->hi_max, w_hi_max);
+      atomicMin(&tl->lo_min[warp >> 2], w_lo_min);
+      atomicMax(&tl->hi_max[warp >> 2], w_hi_max);
     }
   }
   __syncthreads();
-  const int hi_max = tl->hi_max;
-  const int blk0 = hi_max > 0 ? tl->lo_min / kApmBlock : 0;
-  const int n = hi_max > 0 ? (hi_max + kApmBlock - 1) / kApmBlock - blk0 : 0;  // key blocks
+  // key blocks of each tile, [first, end), and of the CTA
+  auto first_of = [&](int i) { return tl->lo_min[i] / kApmBlock; };
+  auto end_of = [&](int i) { return (tl->hi_max[i] + kApmBlock - 1) / kApmBlock; };
+  const bool none0 = tl->hi_max[0] == 0, none1 = tl->hi_max[1] == 0;  // no live row
+  const int g0 = none0 ? (none1 ? 0 : first_of(1)) : (none1 ? first_of(0) : min(first_of(0), first_of(1)));
+  const int g1 = max(end_of(0), end_of(1));  // 0 without a live row
   volatile int* abort_flag = &tl->abort;
 
   if (warp >= kApmSoftmaxWarps) {
     regs_dec<kApmRegsOther>();
-    if (warp == 16 && n > 0) {
-      // ------------------------------------------------------------ producer
+    if ((warp == 8 || warp == 11) && g1 > g0) {
+      // ---------------------------------------------- producers of K and of V
+      // One lane issues all of a block's boxes, from values that the warp has
+      // in common (boxes issued by several lanes take about 100 cycles each).
+      const int kv = warp == 8 ? 0 : 1;
+      const bool leader = elect_one();
       const uint64_t pol = make_l2_policy_evict_last();  // K and V are read again by other tiles
-      if (lane == 0) {
+      if (kv == 0 && leader) {
         mbar_arrive_expect_tx(&tl->q_full, 4u * (uint32_t)(tt * G) * 128u);
 #pragma unroll 1
-        for (int i = 0; i < 2; ++i)
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h)
-            tma_load_4d(q_smem + i * kApmTileBytes + h * kApmHalf, &tmap_q, &tl->q_full, 0, kvh * G,
-                        tl->t_first + tl->tok0 + i * tt, h);
+        for (int i = 0; i < 4; ++i)
+          tma_load_4d(q_smem + i * kApmHalf, &tmap_q, &tl->q_full, 0, kvh * G, tl->t_first + tl->tok0 + (i >> 1) * tt,
+                      i & 1);
       }
+      __syncwarp();
       const int outside = p.num_blocks * p.tokens_per_block;  // a box there reads zeros
-      int s = 0;
-      uint32_t ph = 0;
-      bool alive = true;
       const int32_t* table = p.block_table + (size_t)seq * p.bt_stride;
-      const int lo_min = tl->lo_min;
-      int next_slot = -1;  // pool token of this lane's page in the next block
-      auto look_up = [&](int b) {
-        const int j = (blk0 + b) * kApmBlock + lane * kApmPage;
+      const int lo_min = min(tl->lo_min[0], tl->lo_min[1]), hi_max = max(tl->hi_max[0], tl->hi_max[1]);
+      // pool token of this lane's page of block g (lanes 0-3), -1 where the lookup failed
+      auto look_up = [&](int g) {
+        const int j = g * kApmBlock + (lane & 3) * kApmPage;
         int v = outside;
-        bool bad = false;
-        if (lane < 8 && j < hi_max && j + kApmPage > lo_min) {
-          const long long sl = apm_slot(p, table, j);
-          bad = sl < 0;
-          if (!bad) v = (int)sl;
-        }
-        const uint32_t m = __ballot_sync(0xffffffffu, bad);
-        if (m != 0 && lane == 0) atomicOr(p.status, kStatusBadBlock);
-        next_slot = v;
-        return m;
+        if (g < g1 && j < hi_max && j + kApmPage > lo_min) v = (int)apm_slot(p, table, j);
+        return v;
       };
+      uint8_t* ring = kv ? v_smem : k_smem;
+      int slot = 0, pool_tok = look_up(g0), next_tok = look_up(g0 + 1);
+      uint32_t ph = 0;
 #pragma unroll 1
-      for (int b = 0; b < n && alive; ++b) {
-        const uint32_t bad = look_up(b);
-        if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&tl->bad[b & 7]) = bad;
-#pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv) {
-          bool got = true;
-          if (2 * b + kv >= kApmStages) got = mbar_wait_warp(&tl->empty[s], ph ^ 1u, abort_flag);
-          if (!got) {
-            if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
-            alive = false;
-            break;
-          }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&tl->full[s], kApmTileBytes);
-            tl->issued = 2 * b + kv + 1;
-          }
-          __syncwarp();
-          if (lane < 8) {
-            uint8_t* dst = kv_smem + (size_t)s * kApmTileBytes + lane * 2048;
-            tma_load_5d(dst, &tmap_kv, &tl->full[s], 0, next_slot, 0, kv, kvh, pol);
-            tma_load_5d(dst + kApmHalf, &tmap_kv, &tl->full[s], 0, next_slot, 1, kv, kvh, pol);
-          }
-          if (++s == kApmStages) {
-            s = 0;
-            ph ^= 1u;
-          }
-        }
-      }
-    } else if (warp == 17 && n > 0) {
-      // ---------------------------------------------------------- UMMA issue
-      // The whole warp walks the loop; one lane issues.
-      constexpr uint32_t kIdescQk = umma_idesc_bf16(128, 128);
-      constexpr uint32_t kIdescPv = umma_idesc_bf16(128, 128) | kUmmaBMnMajor;
-      const bool leader = elect_one();
-      const uint64_t qd = umma_desc_sw128(smem_u32(q_smem));
-      const uint64_t kd = umma_desc_sw128(smem_u32(kv_smem));
-      const uint64_t vd = umma_desc_sw128_mn(smem_u32(kv_smem), kApmHalf);
-      auto qk = [&](int i, int slot) {  // S_i = Q_i K^T, 16 dims a step: 32 bytes of each row
-        const uint64_t ad = qd + (uint64_t)(i * (kApmTileBytes >> 4));
-        const uint64_t bd = kd + (uint64_t)(slot * (kApmTileBytes >> 4));
-        if (leader) {
+      for (int g = g0; g < g1; ++g) {
+        const uint32_t bad = __ballot_sync(0xffffffffu, pool_tok < 0) & 15u;
+        if (pool_tok < 0) pool_tok = outside;
+        int page[4];
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t d = (uint64_t)((kk >> 2) * (kApmHalf >> 4) + (kk & 3) * 2);
-            umma_bf16_ss(tmem + i * 128, ad + d, bd + d, kIdescQk, kk ? 1u : 0u);
-          }
-          umma_commit(&tl->s_full[i]);
+        for (int k = 0; k < 4; ++k) page[k] = __shfl_sync(0xffffffffu, pool_tok, k);
+        pool_tok = next_tok;
+        next_tok = look_up(g + 2);  // two blocks ahead: the lookup is not waited for
+        if (g - g0 >= kApmStages && !mbar_wait_all(&tl->empty[kv][slot], ph ^ 1u, abort_flag)) {
+          if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
+          break;
         }
-      };
-      auto pv = [&](int i, int slot, int h, uint32_t acc) {  // O_i += P_i V over keys 64 h .. 64 h + 63
-        // 16 keys a step: 2048 bytes of V, 8 columns of P
-        const uint64_t bd = vd + (uint64_t)(slot * (kApmTileBytes >> 4) + 512 * h);
         if (leader) {
+          if (kv == 0) {
+            *reinterpret_cast<volatile uint32_t*>(&tl->bad[g & 15]) = bad;
+            if (bad != 0) atomicOr(p.status, kStatusBadBlock);
+          }
+          mbar_arrive_expect_tx(&tl->full[kv][slot], kApmKvBytes);
+          uint8_t* dst = ring + (size_t)slot * kApmKvBytes;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_bf16_ts(tmem + 256 + i * 128, tmem + i * 128 + 32 * h + 8 * kk, bd + 128u * kk, kIdescPv,
-                         kk ? 1u : acc);
+          for (int k = 0; k < 4; ++k) {
+            tma_load_5d(dst + k * 2048, &tmap_kv, &tl->full[kv][slot], 0, page[k], 0, kv, kvh, pol);
+            tma_load_5d(dst + k * 2048 + kApmKvHalf, &tmap_kv, &tl->full[kv][slot], 0, page[k], 1, kv, kvh, pol);
+          }
+          tl->issued[kv] = g - g0 + 1;
         }
-      };
-      auto next = [](int& slot, uint32_t& ph) {
+        __syncwarp();
         if (++slot == kApmStages) {
           slot = 0;
           ph ^= 1u;
         }
-      };
-      int slot = 0;  // ring slot and phase of the load looked at
-      uint32_t ph = 0;
-      bool ok = mbar_wait_warp(&tl->q_full, 0, abort_flag) && mbar_wait_warp(&tl->full[0], 0, abort_flag);
-      if (ok) {
-        tc_fence_after();
-        qk(0, 0);
-        qk(1, 0);
-        if (leader) umma_commit(&tl->empty[0]);
-      } else if (lane == 0) {
-        apm_fail(p, tl, kStatusTimeoutFull);
       }
+    } else if (warp >= 9 && warp <= 10 && g1 > g0) {
+      // ---------------------------------------------------------- UMMA issue
+      // One warp per tile; the whole warp walks the loop, one lane issues.  Step
+      // g: P V of block g, then Q K^T of block g + 2 into the buffer that this
+      // frees.  MMAs of one thread run in the order of their issue.
+      constexpr uint32_t kIdescQk = umma_idesc_bf16(128, 64);
+      constexpr uint32_t kIdescPv = umma_idesc_bf16(128, 128) | kUmmaBMnMajor;
+      const int i = warp - 9;
+      const bool leader = elect_one();
+      const uint64_t qd = umma_desc_sw128(smem_u32(q_smem)) + (uint64_t)(i * (kApmTileBytes >> 4));
+      const uint64_t kd = umma_desc_sw128(smem_u32(k_smem));
+      const uint64_t vd = umma_desc_sw128_mn(smem_u32(v_smem), kApmKvHalf);
+      const bool none = tl->hi_max[i] == 0;
+      const int first = none ? g1 : first_of(i), end = none ? g1 : end_of(i);
+      const uint32_t s_col = tmem + i * 128, o_col = tmem + 256 + i * 128;
+      int k_slot = 0, v_slot = 0;
+      uint32_t k_ph = 0, v_ph = 0;
+      bool ok = mbar_wait_all(&tl->q_full, 0, abort_flag);
+      if (!ok && lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
 #pragma unroll 1
-      for (int b = 0; b < n && ok; ++b) {
-        const bool more = b + 1 < n;
-        next(slot, ph);
-        const int v_slot = slot;
-        ok = mbar_wait_warp(&tl->full[slot], ph, abort_flag);
-        int k_slot = 0;
-        if (more) {
-          next(slot, ph);
-          k_slot = slot;
-          ok = ok && mbar_wait_warp(&tl->full[slot], ph, abort_flag);
-        }
+      for (int g = g0 - 2; g < g1 && ok; ++g) {
+        const int kp = g - first;  // the tile's how-manieth block; its buffer is kp & 1
+        const uint32_t buf = (uint32_t)kp & 1u;
+        const bool has_k = g + 2 < g1, has_v = g >= g0;
+        if (has_k) ok = mbar_wait_all(&tl->full[0][k_slot], k_ph, abort_flag);
+        if (has_v && ok) ok = mbar_wait_all(&tl->full[1][v_slot], v_ph, abort_flag);
         if (!ok) {
           if (lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
           break;
         }
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll 1
-          for (int h = 0; h < 2 && ok; ++h) {
-            ok = mbar_wait_warp(&tl->p_full[i][h], (uint32_t)b & 1u, abort_flag);
-            if (ok) {
-              tc_fence_after();
-              pv(i, v_slot, h, (uint32_t)(b | h) ? 1u : 0u);
-            }
-          }
-          if (!ok) {
+        if (g >= first && g < end) {
+          if (!mbar_wait_all(&tl->p_full[i][buf], (uint32_t)(kp >> 1) & 1u, abort_flag)) {
             if (lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
+            ok = false;
             break;
           }
-          if (leader && i == 1) umma_commit(&tl->empty[v_slot]);
-          if (more) {
-            qk(i, k_slot);
-            if (leader && i == 1) umma_commit(&tl->empty[k_slot]);
-          } else if (leader) {
-            umma_commit(&tl->o_full[i]);
+          tc_fence_after();
+          // O += P V: 16 keys a step, 2048 bytes of V, 8 columns of P
+          const uint64_t bd = vd + (uint64_t)(v_slot * (kApmKvBytes >> 4));
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_bf16_ts(o_col, s_col + buf * 64 + 8 * kk, bd + 128u * kk, kIdescPv, (kp | kk) ? 1u : 0u);
+            umma_commit(g + 1 < end ? &tl->o_done[i] : &tl->o_last[i]);
           }
+          __syncwarp();
+        }
+        if (g + 2 >= first && g + 2 < end) {
+          tc_fence_after();
+          // S = Q K^T: 16 dims a step, 32 bytes of each row
+          const uint64_t bd = kd + (uint64_t)(k_slot * (kApmKvBytes >> 4));
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              umma_bf16_ss(s_col + buf * 64, qd + (uint64_t)((kk >> 2) * (kApmHalf >> 4) + (kk & 3) * 2),
+                           bd + (uint64_t)((kk >> 2) * (kApmKvHalf >> 4) + (kk & 3) * 2), kIdescQk, kk ? 1u : 0u);
+            umma_commit(&tl->s_full[i][buf]);
+          }
+          __syncwarp();
+        }
+        if (leader) {
+          if (has_v) umma_commit(&tl->empty[1][v_slot]);
+          if (has_k) umma_commit(&tl->empty[0][k_slot]);
+        }
+        __syncwarp();
+        if (has_v && ++v_slot == kApmStages) {
+          v_slot = 0;
+          v_ph ^= 1u;
+        }
+        if (has_k && ++k_slot == kApmStages) {
+          k_slot = 0;
+          k_ph ^= 1u;
         }
       }
       if (!ok && leader) {  // what was issued reads shared memory and writes TMEM until it is done
-        umma_commit(&tl->drain);
-        mbar_wait(&tl->drain, 0, nullptr);
+        umma_commit(&tl->drain[i]);
+        mbar_wait(&tl->drain[i], 0, nullptr);
       }
     }
   } else {
     regs_inc<kApmRegsSoftmax>();
     // ------------------------------------------------------------- softmax
+    const int wg = warp >> 2;  // tile
+    const int r = tid & 127;   // row of the tile
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int wg = warp >> 3;       // tile
-    const int u = (warp >> 2) & 1;  // which of the row's two threads
-    const int r = tid & 127;        // row of the tile
-    const uint32_t s_addr = tmem + lanes + wg * 128;
-    const uint32_t o_addr = tmem + lanes + 256 + wg * 128 + 64 * u;  // this thread's half of the row's output
-    const int pair_bar = 1 + wg * 4 + (warp & 3);                    // barrier of the two warps of these rows
+    const uint32_t o_addr = tmem + lanes + 256 + wg * 128;
+    const int first = tl->hi_max[wg] == 0 ? 0 : first_of(wg);
+    const int n = tl->hi_max[wg] == 0 ? 0 : end_of(wg) - first;  // the tile's key blocks
     float m_ref = -INFINITY, l = 0.f;
     float slope2 = 0.f;
     int pos = 0;
@@ -488,26 +457,31 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       if (valid) slope2 = p.mod.slopes[kvh * G + r % G] * 1.4426950408889634f;
     }
     bool ok = true;
+#pragma unroll 1
     for (int b = 0; b < n; ++b) {
-      bool got = mbar_wait_warp(&tl->s_full[wg], (uint32_t)b & 1u, abort_flag);
+      const uint32_t s_addr = tmem + lanes + wg * 128 + (b & 1) * 64;
+      if (!mbar_wait_all(&tl->s_full[wg][b & 1], (uint32_t)(b >> 1) & 1u, abort_flag)) {
+        ok = false;
+        break;
+      }
       tc_fence_after();
-      const int j0 = (blk0 + b) * kApmBlock;
-      const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&tl->bad[b & 7]);
-      const bool partial = j0 < tl->lo_max || j0 + kApmBlock > tl->hi_min;          // for some live row of the CTA
-      const bool masked = j0 < w_lo || j0 + kApmBlock > w_hi || bad != 0;   // for some live row of the warp
-      // this thread's keys: 32 u .. 32 u + 31 (chunk 0) and 64 + 32 u .. (chunk 1)
-      float x[32], x1[32];
-      tmem_ld32_nowait(s_addr + 64 + 32 * u, x1);
-      tmem_ld32_nowait(s_addr + 32 * u, x);
-      if (partial && got) {
-        // partly visible block: V values that are not finite to zero
-        const int m = 2 * b + 1;
-        got = mbar_wait_warp(&tl->full[m % kApmStages], (uint32_t)(m / kApmStages) & 1u, abort_flag);
-        uint4* v = reinterpret_cast<uint4*>(kv_smem + (size_t)(m % kApmStages) * kApmTileBytes);
+      const int g = first + b, j0 = g * kApmBlock;
+      float x[64];
+      tmem_ld32_nowait(s_addr, x);
+      tmem_ld32_nowait(s_addr + 32, x + 32);
+      const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&tl->bad[g & 15]);
+      const bool masked = j0 < w_lo || j0 + kApmBlock > w_hi || bad != 0;  // for some live row of the warp
+      if (j0 < tl->lo_max || j0 + kApmBlock > tl->hi_min) {
+        // not visible to all live rows of the CTA: V values that are not finite to zero
+        const int m = g - g0;
+        if (!mbar_wait_warp(&tl->full[1][m % kApmStages], (uint32_t)(m / kApmStages) & 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        uint4* v = reinterpret_cast<uint4*>(v_smem + (size_t)(m % kApmStages) * kApmKvBytes);
 #pragma unroll 4
         for (int i = 0; i < 8; ++i) {
-          const int at = i * 256 + (tid & 255);
-          uint4 q = v[at];
+          uint4 q = v[i * 128 + r];
           if ((not_finite2(q.x) | not_finite2(q.y) | not_finite2(q.z) | not_finite2(q.w)) != 0) {
             *reinterpret_cast<volatile int*>(&tl->poison) = 1;
             __threadfence_block();
@@ -515,102 +489,90 @@ __global__ void __launch_bounds__(kApmThreads, 1)
               const uint32_t f = not_finite2(w);
               return w & ((f & 0x8000u ? 0u : 0xFFFFu) | (f & 0x80000000u ? 0u : 0xFFFF0000u));
             };
-            v[at] = make_uint4(clean(q.x), clean(q.y), clean(q.z), clean(q.w));
+            v[i * 128 + r] = make_uint4(clean(q.x), clean(q.y), clean(q.z), clean(q.w));
           }
         }
-        // the tensor core sees the values written; P V starts when all eight
+        // the tensor core sees the values written; P V starts when all four
         // warps have reported their P, so after all of the block is clean
         fence_proxy_async_smem();
       }
       tmem_wait_ld();
-      // ---- modifications (base 2) of one chunk
-      bool small = false;  // every |score| of the warp is within the cap's polynomial
-      auto modify = [&](float* y, int h) {
-        if (CAP) {
-          if (small) {
-            f32x2 pc[5];
-#pragma unroll
-            for (int k = 0; k < 5; ++k) pc[k] = pack2(p.mod.poly[k], p.mod.poly[k]);
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              const f32x2 v = pack2(y[c], y[c + 1]);
-              unpack2(mul2(v, cap_poly(mul2(v, v), pc)), y[c], y[c + 1]);
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) y[c] = cap_score(y[c], p.mod.cap_in, p.mod.cap2);
-          }
-        }
-        const int k0 = j0 + 64 * h + 32 * u;  // position of the chunk's first key
-        if (BIAS) {
-          const float d0 = (float)(k0 - pos);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) y[c] = fmaf(-slope2, fabsf(d0 + (float)c), CAP ? y[c] : y[c] * p.mod.mul);
-        }
-        if (masked) {
-          const int v0 = lo - k0, v1 = hi - k0;
-          const uint32_t pages = bad >> (4 * h + 2 * u);
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (c < v0 || c >= v1 || ((pages >> (c / kApmPage)) & 1u)) y[c] = -INFINITY;
-        }
-      };
-      auto max_of = [](const float* y) {
-        float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          m0 = max3(m0, y[c], y[c + 1]);
-          m1 = max3(m1, y[c + 2], y[c + 3]);
-        }
-        return fmaxf(m0, m1);
-      };
-      // `direct`: scores stay q . k, the cap's polynomial enters in the exponent
-      bool direct = false;
-      float m_new;
+      // ---- modifications (base 2).  `direct`: scores stay q . k, and the scale
+      // or the cap's polynomial enters in the exponent
+      bool direct = !CAP && !BIAS;
+      float m_new = -INFINITY;
       if (CAP) {
         float a0 = 0.f, a1 = 0.f;
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
+        for (int c = 0; c < 64; c += 4) {
           a0 = max3(a0, fabsf(x[c]), fabsf(x[c + 1]));
-          a1 = max3(a1, fabsf(x1[c]), fabsf(x1[c + 1]));
+          a1 = max3(a1, fabsf(x[c + 2]), fabsf(x[c + 3]));
         }
         a0 = fmaxf(a0, a1);
-        small = !__any_sync(0xffffffffu, !(a0 <= p.mod.poly_max));
+        const bool small = !__any_sync(0xffffffffu, !(a0 <= p.mod.poly_max));
         direct = !BIAS && small && !masked && p.mod.cap2 * 0.605f <= kApmBound;
-        const float w = a0 * a0;
-        m_new = a0 * fmaf(fmaf(fmaf(fmaf(p.mod.poly[4], w, p.mod.poly[3]), w, p.mod.poly[2]), w, p.mod.poly[1]), w,
-                          p.mod.poly[0]);
-      }
-      if (!direct) {
-        modify(x1, 1);
-        m_new = max_of(x1);
-        modify(x, 0);
-        m_new = fmaxf(m_new, max_of(x));
-        if (!CAP && !BIAS) m_new *= p.mod.mul;
-      }
-      // ---- the row's reference.  The barrier also orders: both threads hold
-      // their scores before either writes P over them
-      if (named_bar_any(pair_bar, 64, !got || m_new > m_ref + kApmLazy)) {
-        tl->row_x[wg][u][r] = m_new;
-        if (named_bar_any(pair_bar, 64, !got)) {
-          if (lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
-          ok = false;
-          break;
+        if (direct) {
+          const float w = a0 * a0;
+          m_new = a0 * fmaf(fmaf(fmaf(fmaf(p.mod.poly[4], w, p.mod.poly[3]), w, p.mod.poly[2]), w, p.mod.poly[1]), w,
+                            p.mod.poly[0]);
+        } else if (small) {
+          f32x2 pc[5];
+#pragma unroll
+          for (int k = 0; k < 5; ++k) pc[k] = pack2(p.mod.poly[k], p.mod.poly[k]);
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) {
+            const f32x2 v = pack2(x[c], x[c + 1]);
+            unpack2(mul2(v, cap_poly(mul2(v, v), pc)), x[c], x[c + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) x[c] = cap_score(x[c], p.mod.cap_in, p.mod.cap2);
         }
-        m_new = fmaxf(m_new, tl->row_x[wg][u ^ 1][r]);
-        const bool grow = m_new > m_ref + kApmLazy;  // also from -inf
+      }
+      if (BIAS) {
+        const float d0 = (float)(j0 - pos);
+#pragma unroll
+        for (int c = 0; c < 64; ++c) x[c] = fmaf(-slope2, fabsf(d0 + (float)c), CAP ? x[c] : x[c] * p.mod.mul);
+      }
+      if (masked) {
+        const int v0 = lo - j0, v1 = hi - j0;
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c < v0 || c >= v1 || ((bad >> (c / kApmPage)) & 1u)) x[c] = -INFINITY;
+      }
+      if (!(CAP && direct)) {
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          mx[0] = max3(mx[0], x[c], x[c + 1]);
+          mx[1] = max3(mx[1], x[c + 2], x[c + 3]);
+        }
+        m_new = fmaxf(mx[0], mx[1]);
+        if (direct) m_new *= p.mod.mul;
+      }
+      // ---- the row's reference
+      const bool grow = m_new > m_ref + kApmLazy;  // also from -inf
+      if (__any_sync(0xffffffffu, grow)) {
         const float f = grow ? ex2(m_ref - m_new) : 1.f;
         if (grow) m_ref = m_new;
         l *= f;
-        if (b > 0 && __any_sync(0xffffffffu, grow)) {
+        if (b > 0) {
+          // the previous block's P V may still run (the one before it is done: S
+          // of this block was computed after it)
+          if (!mbar_wait_warp(&tl->o_done[wg], (uint32_t)(b - 1) & 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t v[16];
-            tmem_ld16_nowait(o_addr + 16 * c, v);
+            float v[32];
+            uint32_t w[32];
+            tmem_ld32_nowait(o_addr + 32 * c, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-            tmem_st16(o_addr + 16 * c, v);
+            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * f);
+            tmem_st32(o_addr + 32 * c, w);
           }
         }
       }
@@ -618,75 +580,62 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       const float neg = m_ref == -INFINITY ? 0.f : -m_ref;  // nothing seen yet: weights 0, NaN stays NaN
       const f32x2 neg2 = pack2(neg, neg);
       f32x2 sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+      uint32_t pk[32];
+      if (CAP && direct) {
+        f32x2 pc[5];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h == 1) {  // P lies in the columns of keys 0-63: the second chunk's scores are still there
-          tmem_ld32_nowait(s_addr + 64 + 32 * u, x);
-          tmem_wait_ld();
-          if (!direct && (CAP || BIAS || masked)) modify(x, 1);
+        for (int k = 0; k < 5; ++k) pc[k] = pack2(p.mod.poly[k], p.mod.poly[k]);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const f32x2 v = pack2(x[2 * c], x[2 * c + 1]);
+          float e0, e1;
+          unpack2(fma2(v, cap_poly(mul2(v, v), pc), neg2), e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
+          pk[c] = pack_bf16x2(e0, e1);
         }
-        uint32_t pk[16];
-        if (CAP && direct) {
-          f32x2 pc[5];
+      } else {
+        const f32x2 mul_2 = pack2(p.mod.mul, p.mod.mul);
 #pragma unroll
-          for (int k = 0; k < 5; ++k) pc[k] = pack2(p.mod.poly[k], p.mod.poly[k]);
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const f32x2 v = pack2(x[2 * c], x[2 * c + 1]);
-            float e0, e1;
-            unpack2(fma2(v, cap_poly(mul2(v, v), pc), neg2), e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-            sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
-            pk[c] = pack_bf16x2(e0, e1);
-          }
-        } else {
-          const f32x2 mul_2 = pack2(p.mod.mul, p.mod.mul);
-          const bool poly = !CAP && !masked;
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            f32x2 y = pack2(x[2 * c], x[2 * c + 1]);
-            y = (CAP || BIAS) ? add2(y, neg2) : fma2(y, mul_2, neg2);
-            float e0, e1;
-            if (poly && (c & 3) == 3) {
-              ex2_poly2(y, e0, e1);
-            } else {
-              unpack2(y, e0, e1);
-              e0 = ex2(e0);
-              e1 = ex2(e1);
-            }
-            sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
-            pk[c] = pack_bf16x2(e0, e1);
-          }
+        for (int c = 0; c < 32; ++c) {
+          f32x2 y = pack2(x[2 * c], x[2 * c + 1]);
+          y = (CAP || BIAS) ? add2(y, neg2) : fma2(y, mul_2, neg2);
+          float e0, e1;
+          unpack2(y, e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
+          pk[c] = pack_bf16x2(e0, e1);
         }
-        tmem_st16(s_addr + 32 * h + 16 * u, pk);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tl->p_full[wg][h]);
       }
+      tmem_st32(s_addr, pk);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tl->p_full[wg][b & 1]);
       float s0, s1;
       unpack2(add2(sum2[0], sum2[1]), s0, s1);
       l += s0 + s1;
     }
     // ------------------------------------------------------------ epilogue
-    if (n > 0 && ok) ok = mbar_wait_warp(&tl->o_full[wg], 0, abort_flag);
+    if (n > 0 && ok) ok = mbar_wait_warp(&tl->o_last[wg], 0, abort_flag);
     tc_fence_after();
-    tl->row_x[wg][u][r] = l;
-    if (named_bar_any(pair_bar, 64, !ok)) {
+    // the output is staged where the tile's Q was: all its Q K^T are done, or
+    // there were none and the load only has to have landed
+    if (n == 0 && g1 > g0) ok = mbar_wait_warp(&tl->q_full, 0, abort_flag);
+    if (!ok) {
       if (lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
     } else {
-      l += tl->row_x[wg][u ^ 1][r];
       const int seq = tl->seq, t_first = tl->t_first, q_len = tl->q_len, tok0 = tl->tok0 + wg * tt;
-      const int kvh = (int)(blockIdx.x % (unsigned)p.n_kv_heads);
       const bool dead = !live || n == 0;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      // the row's output to shared memory (the Q tile is not read any more):
-      // 16-byte pieces, 128-byte swizzle, then whole rows to global memory
-      uint8_t* half_smem = q_smem + wg * kApmTileBytes + u * kApmHalf;
+      // the row's output to shared memory: 16-byte pieces, 128-byte swizzle,
+      // then whole rows to global memory
+      uint8_t* tile_smem = q_smem + wg * kApmTileBytes;
       const bool poison = n > 0 && *reinterpret_cast<volatile int*>(&tl->poison) != 0;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 4; ++c) {
         float v[32];
         if (n > 0) {
           tmem_ld32_nowait(o_addr + 32 * c, v);
@@ -696,13 +645,13 @@ __global__ void __launch_bounds__(kApmThreads, 1)
         for (int i = 0; i < 32; ++i) v[i] = dead ? 0.f : v[i] * inv;
         if (poison && live) {
           for (int b = 0; b < n; ++b) {
-            const int j0 = (blk0 + b) * kApmBlock;
+            const int j0 = (first + b) * kApmBlock;
             if (j0 >= tl->lo_max && j0 + kApmBlock <= tl->hi_min) continue;  // not cleaned
             for (int j = max(lo, j0); j < min(hi, j0 + kApmBlock); ++j) {
               const long long sl = apm_slot(p, p.block_table + (size_t)seq * p.bt_stride, j);
               if (sl < 0) continue;
               const __nv_bfloat16* vr =
-                  p.pool + ((size_t)sl * 2 * p.n_kv_heads + p.n_kv_heads + kvh) * kHeadDim + 64 * u + 32 * c;
+                  p.pool + ((size_t)sl * 2 * p.n_kv_heads + p.n_kv_heads + kvh) * kHeadDim + 32 * c;
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 const float f = __bfloat162float(vr[i]);
@@ -715,22 +664,24 @@ __global__ void __launch_bounds__(kApmThreads, 1)
         for (int i = 0; i < 4; ++i) {
           const uint4 w = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
                                      pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
-          *reinterpret_cast<uint4*>(half_smem + r * 128 + (((4 * c + i) ^ (r & 7)) << 4)) = w;
+          *reinterpret_cast<uint4*>(tile_smem + (c >> 1) * kApmHalf + r * 128 + ((((c & 1) * 4 + i) ^ (r & 7)) << 4)) =
+              w;
         }
       }
-      if (valid && p.lse && u == 0)
+      if (valid && p.lse)
         p.lse[(size_t)(t_first + tok0 + r / G) * p.lse_stride + kvh * G + r % G] =
             (dead || l == 0.f) ? -INFINITY : (m_ref == -INFINITY ? l : (m_ref + log2f(l)) * kLn2);
       __syncwarp();
       const int r0 = (warp & 3) * 32;
 #pragma unroll 4
-      for (int it = 0; it < 8; ++it) {
-        const int rr = r0 + 4 * it + (lane >> 3), ch = lane & 7;
+      for (int it = 0; it < 16; ++it) {
+        const int rr = r0 + 2 * it + (lane >> 4), ch = lane & 15;
         const int tk = tok0 + rr / G;
         if (seq >= 0 && rr < tt * G && tk < q_len) {
-          const uint4 w = *reinterpret_cast<const uint4*>(half_smem + rr * 128 + ((ch ^ (rr & 7)) << 4));
+          const uint4 w = *reinterpret_cast<const uint4*>(tile_smem + (ch >> 3) * kApmHalf + rr * 128 +
+                                                          (((ch & 7) ^ (rr & 7)) << 4));
           *reinterpret_cast<uint4*>(p.out + (size_t)(t_first + tk) * p.out_stride +
-                                    (size_t)(kvh * G + rr % G) * kHeadDim + 64 * u + ch * 8) = w;
+                                    (size_t)(kvh * G + rr % G) * kHeadDim + ch * 8) = w;
         }
       }
     }
@@ -740,12 +691,12 @@ __global__ void __launch_bounds__(kApmThreads, 1)
   if (tl->abort && tid == 0) {
     // loads still in flight land (bounded waits) before the CTA's memory goes
     mbar_wait(&tl->q_full, 0, nullptr);
-    const int end = tl->issued;
-    for (int m = end > kApmStages ? end - kApmStages : 0; m < end; ++m)
-      mbar_wait(&tl->full[m % kApmStages], (uint32_t)(m / kApmStages) & 1u, nullptr);
+    for (int kv = 0; kv < 2; ++kv)
+      for (int m = max(0, tl->issued[kv] - kApmStages); m < tl->issued[kv]; ++m)
+        mbar_wait(&tl->full[kv][m % kApmStages], (uint32_t)(m / kApmStages) & 1u, nullptr);
   }
   __syncthreads();
-  if (warp == 17) {
+  if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

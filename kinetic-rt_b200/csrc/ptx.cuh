@@ -342,6 +342,14 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
 }
 
+// The same polled by every lane: no exchange when the phase is complete
+// already.  All lanes of the warp see the same barrier; the result is made
+// uniform once a wait was needed.
+__device__ __forceinline__ bool mbar_wait_all(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return mbar_wait_warp(bar, parity, abort);
+}
+
 // Wait for data that other CTAs of the cluster send into this CTA's shared
 // memory.  The senders always send, also after their own failures, so this
 // wait ignores the CTA's abort flag (the CTA must not exit while copies may
