@@ -13,13 +13,14 @@ namespace krt {
 
 struct ScoreMod {
   float mul;         // scale * log2(e)
+  float2 mul2;       // the same twice
   float cap2;        // cap * log2(e), 0 = no cap
   float cap_in;      // 2 * log2(e) * scale / cap: ex2(s * cap_in) = e^(2 x / c)
   const float* slopes;  // [n_heads] or NULL
   int window;        // 0 = none
-  // cap by polynomial while |s| <= poly_max: x = s * P(s^2), see cap_poly
-  float poly[5];
-  float poly_max;    // negative: never
+  // cap by polynomial while s^2 <= poly_max2: x = s * P(s^2), see cap_poly
+  float2 poly[5];    // each coefficient twice: operands of packed multiply-adds
+  float poly_max2;   // negative: never
 };
 
 inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, int window) {
@@ -27,21 +28,23 @@ inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, 
   ScoreMod m;
   const float sc = scale > 0.f ? scale : 0.08838834764831845f;  // 1 / sqrt(128)
   m.mul = sc * kLog2e;
+  m.mul2 = make_float2(m.mul, m.mul);
   m.cap2 = softcap * kLog2e;
   m.cap_in = softcap > 0.f ? 2.f * kLog2e * sc / softcap : 0.f;
   m.slopes = slopes;
   m.window = window;
   // cap2 * tanh(u), u = a s, as an odd polynomial in s (cap_poly's coefficients times cap2 a^(2k+1));
   // left out where powers of a could leave the range of a float
-  m.poly_max = -1.f;
+  m.poly_max2 = -1.f;
+  for (int k = 0; k < 5; ++k) m.poly[k] = make_float2(0.f, 0.f);
   if (softcap > 0.f) {
     static const double c[5] = {0.9999985098838806, -0.33326974511146545, 0.13257454335689545, -0.05019525811076164,
                                 0.013194185681641102};
     const double a = (double)sc / softcap;
     if (a > 1e-4 && a < 1e3 && softcap < 1e6f) {
       double f = a * m.cap2;
-      for (int k = 0; k < 5; ++k, f *= a * a) m.poly[k] = (float)(c[k] * f);
-      m.poly_max = (float)(0.7 / a);
+      for (int k = 0; k < 5; ++k, f *= a * a) m.poly[k] = make_float2((float)(c[k] * f), (float)(c[k] * f));
+      m.poly_max2 = (float)(0.7 / a * (0.7 / a));
     }
   }
   return m;
@@ -72,6 +75,7 @@ __device__ __forceinline__ float cap_score(float s, float cap_in, float cap2) {
 
 // ---- two floats in one 64-bit register: one issue slot for two multiply-adds
 typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(const float2& v) { return *reinterpret_cast<const f32x2*>(&v); }
 __device__ __forceinline__ f32x2 pack2(float lo, float hi) {
   f32x2 r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -107,8 +111,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // by at most 9.5e-8.  Scores beyond that take cap_score.  Five multiply-adds
 // and no special-function operation, of which the softmax needs all: tanh by
 // ex2 and rcp would triple them.
-__device__ __forceinline__ f32x2 cap_poly(f32x2 w, const f32x2* c) {
-  return fma2(fma2(fma2(fma2(c[4], w, c[3]), w, c[2]), w, c[1]), w, c[0]);
+__device__ __forceinline__ f32x2 cap_poly(f32x2 w, const float2* c) {
+  return fma2(fma2(fma2(fma2(pair_of(c[4]), w, pair_of(c[3])), w, pair_of(c[2])), w, pair_of(c[1])), w, pair_of(c[0]));
+}
+// The same for one value, times s: the capped score of s = sqrt(w).
+__device__ __forceinline__ float cap_at(float w, const float2* c) {
+  return sqrtf(w) * fmaf(fmaf(fmaf(fmaf(c[4].x, w, c[3].x), w, c[2].x), w, c[1].x), w, c[0].x);
 }
 
 }  // namespace krt

@@ -87,6 +87,7 @@ struct ApmParams {
   int* status;
   int num_tokens, num_seqs, bt_stride, num_blocks, tokens_per_block;
   int n_kv_heads, group, tile_tokens;  // tile_tokens = 128 / group
+  uint32_t group_inv;                  // row / group = row * group_inv >> 16 for rows below 128
   int out_stride, lse_stride;
   ScoreMod mod;
 };
@@ -104,11 +105,8 @@ struct ApmSmemTail {
   int issued[2];          // blocks of K and V requested
   int abort;
   int poison;             // a V value that is not finite was taken out of a partly visible block
-  int seq, tile;          // this CTA's work
-  int t_first, q_len, tok0, pos0;  // first row and rows of the sequence, first token of the tiles, position of token 0
   int lo_min[2], hi_max[2];        // per tile, over its live rows
   int lo_max, hi_min;              // over the CTA's live rows
-  int scan[kApmThreads / 32];
   uint32_t bad[16];       // per block (ring): pages that could not be looked up
 };
 
@@ -122,17 +120,8 @@ __device__ __forceinline__ void apm_fail(const ApmParams& p, ApmSmemTail* tl, in
   *reinterpret_cast<volatile int*>(&tl->abort) = 1;
 }
 
-// Register split after the prologue: 384 threads start with 168 registers each
-// (64512); 256 x 216 + 128 x 72 = 64512.
-constexpr int kApmRegsSoftmax = 216;
-constexpr int kApmRegsOther = 72;
-template <int N>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+__device__ __forceinline__ f32x2 cap_poly_r(f32x2 w, const f32x2* c) {
+  return fma2(fma2(fma2(fma2(c[4], w, c[3]), w, c[2]), w, c[1]), w, c[0]);
 }
 
 // Exponent bits all ones in either bf16 half of w: a 1 in bit 15 or 31.
@@ -163,7 +152,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.group, tt = p.tile_tokens;
 
-  if (tid == 0) {
+  if (warp == 8 && lane == 0) {  // (the warp that uses q_full before the others see it)
     for (int i = 0; i < 2; ++i) {
       for (int s = 0; s < kApmStages; ++s) {
         mbar_init(&tl->full[i][s], 1);
@@ -184,7 +173,6 @@ __global__ void __launch_bounds__(kApmThreads, 1)
     fence_mbar_init();
     tl->abort = 0;
     tl->poison = 0;
-    tl->seq = -1;
     tl->lo_max = 0;
     tl->hi_min = INT_MAX;
     tma_prefetch_desc(&tmap_q);
@@ -198,80 +186,84 @@ __global__ void __launch_bounds__(kApmThreads, 1)
   pdl_launch_dependents();
 
   // ---- this CTA's (sequence, pair of tiles): sequences in order, the last
-  // (heaviest) tokens of each first, KV heads innermost
+  // (heaviest) tokens of each first, KV heads innermost.  Every warp finds it
+  // by itself, 128 sequences at a time, so that their loads overlap.
   const int kvh = (int)(blockIdx.x % (unsigned)p.n_kv_heads);
   const int target = (int)(blockIdx.x / (unsigned)p.n_kv_heads);
+  int seq = -1, t_first = 0, q_len = 0, pos0 = 0, tok0 = 0;
   {
     int base = 0;
-    for (int s0 = 0; s0 < p.num_seqs; s0 += kApmThreads) {
-      const int s = s0 + tid;
-      int n = 0;
-      if (s < p.num_seqs) {
-        int a = p.q_start[s], e = p.q_start[s + 1];
-        if (a < 0 || e > p.num_tokens || e < a) {
-          if (blockIdx.x == 0) atomicOr(p.status, kStatusBadBlock);
-        }
-        a = max(a, 0);
-        e = min(e, p.num_tokens);
-        if (e > a) n = (e - a + 2 * tt - 1) / (2 * tt);
-      }
-      int incl = n;
+#pragma unroll 1
+    for (int s0 = 0; s0 < p.num_seqs && seq < 0; s0 += 128) {
+      int a[4], e[4], p0[4];
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += v;
+      for (int k = 0; k < 4; ++k) {
+        const int s = s0 + 32 * k + lane;
+        const bool in = s < p.num_seqs;
+        a[k] = in ? p.q_start[s] : 0;
+        e[k] = in ? p.q_start[s + 1] : 0;
+        p0[k] = in ? p.q_pos0[s] : 0;
       }
-      __syncthreads();
-      if (lane == 31) tl->scan[warp] = incl;
-      __syncthreads();
-      int before = base, total = base;
-      for (int w = 0; w < kApmThreads / 32; ++w) {
-        if (w < warp) before += tl->scan[w];
-        total += tl->scan[w];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (s0 + 32 * k >= p.num_seqs) break;
+        if (warp == 0 && (a[k] < 0 || e[k] > p.num_tokens || e[k] < a[k]))
+          atomicOr(p.status, kStatusBadBlock);
+        a[k] = max(a[k], 0);
+        e[k] = min(e[k], p.num_tokens);
+        const int n = e[k] > a[k] ? (e[k] - a[k] + 2 * tt - 1) / (2 * tt) : 0;
+        int incl = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, incl, d);
+          if (lane >= d) incl += v;
+        }
+        const int excl = base + incl - n;
+        const uint32_t hit = __ballot_sync(0xffffffffu, target >= excl && target < excl + n);
+        if (hit != 0) {
+          const int who = __ffs(hit) - 1;
+          seq = s0 + 32 * k + who;
+          t_first = __shfl_sync(0xffffffffu, a[k], who);
+          q_len = __shfl_sync(0xffffffffu, e[k], who) - t_first;
+          pos0 = __shfl_sync(0xffffffffu, p0[k], who);
+          tok0 = (__shfl_sync(0xffffffffu, n, who) - 1 - (target - __shfl_sync(0xffffffffu, excl, who))) * 2 * tt;
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
       }
-      const int excl = before + incl - n;
-      if (target >= excl && target < excl + n) {
-        tl->seq = s;
-        tl->tile = n - 1 - (target - excl);
-      }
-      base = total;
-      if (target < base) break;  // uniform
     }
+  }
+  __syncwarp();  // warp 8: q_full is initialised
+  if (warp == 8 && seq >= 0 && elect_one()) {
+    // the queries; keys and values follow when the blocks that are seen are known
+    mbar_arrive_expect_tx(&tl->q_full, 4u * (uint32_t)(tt * G) * 128u);
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i)
+      tma_load_4d(q_smem + i * kApmHalf, &tmap_q, &tl->q_full, 0, kvh * G, t_first + tok0 + (i >> 1) * tt, i & 1);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tl->tmem_base;
-  const int seq = tl->seq;
 
-  // ---- bounds of every row, and of the CTA
+  // ---- bounds of every row, of the warp, of the tiles and of the CTA
   int lo = 0, hi = INT_MAX;  // this row's; rows that are not live stay unmasked, their result is not used
   bool live = false, valid = false;
   int w_lo, w_hi;            // largest lo and smallest hi of the warp's live rows
+  int lo_max, hi_min;        // and of the CTA's
+  int first[2], end[2];      // key blocks of each tile, [first, end); both 0 without a live row
+  int lo_all, hi_all;        // keys that some live row of the CTA sees
   {
-    int t_first = 0, q_len = 0, pos0 = 0, tok0 = 0;
-    if (seq >= 0) {
-      t_first = max(p.q_start[seq], 0);
-      q_len = min(p.q_start[seq + 1], p.num_tokens) - t_first;
-      pos0 = p.q_pos0[seq];
-      tok0 = tl->tile * 2 * tt;
-    }
     const bool pos_ok = pos0 >= 0 && pos0 <= kApmMaxPos && q_len <= kApmMaxPos;
-    if (tid == 0) {
-      tl->t_first = t_first;
-      tl->q_len = q_len;
-      tl->tok0 = tok0;
-      tl->pos0 = pos0;
-      if (!pos_ok) atomicOr(p.status, kStatusBadBlock);
-    }
-    const int r = tid & 127, tok = tok0 + (warp >> 2) * tt + r / G;
+    if (tid == 0 && !pos_ok) atomicOr(p.status, kStatusBadBlock);
+    const int prefix = p.prefix_lens && seq >= 0 ? p.prefix_lens[seq] : 0;
+    // what the query at position `at` sees, apart from kv_start: monotonous in `at`
+    auto lowest = [&](int at) { return p.mod.window > 0 ? max(0, at - p.mod.window + 1) : 0; };
+    auto highest = [&](int at) { return min(pos0 + q_len, max(at + 1, prefix)); };
+    const int r = tid & 127, tok = tok0 + (warp >> 2) * tt + (int)(r * p.group_inv >> 16);
     valid = seq >= 0 && warp < kApmSoftmaxWarps && r < tt * G && tok < q_len;
     if (valid && pos_ok) {
-      const int pos = pos0 + tok;
-      int l = p.kv_start ? p.kv_start[t_first + tok] : 0;
-      if (p.mod.window > 0) l = max(l, pos - p.mod.window + 1);
-      l = max(l, 0);
-      const int h = min(pos0 + q_len, max(pos + 1, p.prefix_lens ? p.prefix_lens[seq] : 0));
+      const int l = max(lowest(pos0 + tok), p.kv_start ? p.kv_start[t_first + tok] : 0);
+      const int h = highest(pos0 + tok);
       live = l < h;
       if (live) {
         lo = l;
@@ -280,26 +272,53 @@ __global__ void __launch_bounds__(kApmThreads, 1)
     }
     w_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0);
     w_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);
-    const int w_lo_min = __reduce_min_sync(0xffffffffu, live ? lo : INT_MAX);
-    const int w_hi_max = __reduce_max_sync(0xffffffffu, live ? hi : 0);
-    if (warp < kApmSoftmaxWarps && lane == 0) {
-      atomicMax(&tl->lo_max, w_lo);
-      atomicMin(&tl->hi_min, w_hi);
-      atomicMin(&tl->lo_min[warp >> 2], w_lo_min);
-      atomicMax(&tl->hi_max[warp >> 2], w_hi_max);
+    int lo_min[2], hi_max[2];
+    if (p.kv_start == nullptr) {
+      // every row is live, and the tiles' first and last tokens have the extremes
+      lo_max = 0;
+      hi_min = INT_MAX;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int from = tok0 + i * tt, to = min(from + tt, q_len) - 1;
+        const bool some = pos_ok && from <= to;
+        lo_min[i] = some ? lowest(pos0 + from) : INT_MAX;
+        hi_max[i] = some ? highest(pos0 + to) : 0;
+        if (some) {
+          lo_max = lowest(pos0 + to);
+          if (hi_min == INT_MAX) hi_min = highest(pos0 + from);
+        }
+      }
+    } else {
+      const int w_lo_min = __reduce_min_sync(0xffffffffu, live ? lo : INT_MAX);
+      const int w_hi_max = __reduce_max_sync(0xffffffffu, live ? hi : 0);
+      if (warp < kApmSoftmaxWarps && lane == 0) {
+        atomicMax(&tl->lo_max, w_lo);
+        atomicMin(&tl->hi_min, w_hi);
+        atomicMin(&tl->lo_min[warp >> 2], w_lo_min);
+        atomicMax(&tl->hi_max[warp >> 2], w_hi_max);
+      }
+      __syncthreads();
+      lo_max = tl->lo_max;
+      hi_min = tl->hi_min;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        lo_min[i] = tl->lo_min[i];
+        hi_max[i] = tl->hi_max[i];
+      }
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      first[i] = hi_max[i] > 0 ? lo_min[i] / kApmBlock : 0;
+      end[i] = hi_max[i] > 0 ? (hi_max[i] + kApmBlock - 1) / kApmBlock : 0;
+    }
+    lo_all = min(lo_min[0], lo_min[1]);
+    hi_all = max(hi_max[0], hi_max[1]);
   }
-  __syncthreads();
-  // key blocks of each tile, [first, end), and of the CTA
-  auto first_of = [&](int i) { return tl->lo_min[i] / kApmBlock; };
-  auto end_of = [&](int i) { return (tl->hi_max[i] + kApmBlock - 1) / kApmBlock; };
-  const bool none0 = tl->hi_max[0] == 0, none1 = tl->hi_max[1] == 0;  // no live row
-  const int g0 = none0 ? (none1 ? 0 : first_of(1)) : (none1 ? first_of(0) : min(first_of(0), first_of(1)));
-  const int g1 = max(end_of(0), end_of(1));  // 0 without a live row
+  const int g0 = hi_all > 0 ? lo_all / kApmBlock : 0;
+  const int g1 = hi_all > 0 ? (hi_all + kApmBlock - 1) / kApmBlock : 0;
   volatile int* abort_flag = &tl->abort;
 
   if (warp >= kApmSoftmaxWarps) {
-    regs_dec<kApmRegsOther>();
     if ((warp == 8 || warp == 11) && g1 > g0) {
       // ---------------------------------------------- producers of K and of V
       // One lane issues all of a block's boxes, from values that the warp has
@@ -307,22 +326,13 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       const int kv = warp == 8 ? 0 : 1;
       const bool leader = elect_one();
       const uint64_t pol = make_l2_policy_evict_last();  // K and V are read again by other tiles
-      if (kv == 0 && leader) {
-        mbar_arrive_expect_tx(&tl->q_full, 4u * (uint32_t)(tt * G) * 128u);
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i)
-          tma_load_4d(q_smem + i * kApmHalf, &tmap_q, &tl->q_full, 0, kvh * G, tl->t_first + tl->tok0 + (i >> 1) * tt,
-                      i & 1);
-      }
-      __syncwarp();
       const int outside = p.num_blocks * p.tokens_per_block;  // a box there reads zeros
       const int32_t* table = p.block_table + (size_t)seq * p.bt_stride;
-      const int lo_min = min(tl->lo_min[0], tl->lo_min[1]), hi_max = max(tl->hi_max[0], tl->hi_max[1]);
       // pool token of this lane's page of block g (lanes 0-3), -1 where the lookup failed
       auto look_up = [&](int g) {
         const int j = g * kApmBlock + (lane & 3) * kApmPage;
         int v = outside;
-        if (g < g1 && j < hi_max && j + kApmPage > lo_min) v = (int)apm_slot(p, table, j);
+        if (g < g1 && j < hi_all && j + kApmPage > lo_all) v = (int)apm_slot(p, table, j);
         return v;
       };
       uint8_t* ring = kv ? v_smem : k_smem;
@@ -370,11 +380,11 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       constexpr uint32_t kIdescPv = umma_idesc_bf16(128, 128) | kUmmaBMnMajor;
       const int i = warp - 9;
       const bool leader = elect_one();
-      const uint64_t qd = umma_desc_sw128(smem_u32(q_smem)) + (uint64_t)(i * (kApmTileBytes >> 4));
-      const uint64_t kd = umma_desc_sw128(smem_u32(k_smem));
-      const uint64_t vd = umma_desc_sw128_mn(smem_u32(v_smem), kApmKvHalf);
-      const bool none = tl->hi_max[i] == 0;
-      const int first = none ? g1 : first_of(i), end = none ? g1 : end_of(i);
+      const uint32_t qd = umma_desc_lo(smem_u32(q_smem)) + i * (kApmTileBytes >> 4);
+      const uint32_t kd = umma_desc_lo(smem_u32(k_smem));
+      const uint32_t vd = umma_desc_lo_mn(smem_u32(v_smem), kApmKvHalf);
+      // (a tile without a live row has no blocks in any step)
+      const int t_end = i == 0 ? end[0] : end[1], t_begin = t_end == 0 ? g1 : (i == 0 ? first[0] : first[1]);
       const uint32_t s_col = tmem + i * 128, o_col = tmem + 256 + i * 128;
       int k_slot = 0, v_slot = 0;
       uint32_t k_ph = 0, v_ph = 0;
@@ -382,7 +392,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       if (!ok && lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
 #pragma unroll 1
       for (int g = g0 - 2; g < g1 && ok; ++g) {
-        const int kp = g - first;  // the tile's how-manieth block; its buffer is kp & 1
+        const int kp = g - t_begin;  // the tile's how-manieth block; its buffer is kp & 1
         const uint32_t buf = (uint32_t)kp & 1u;
         const bool has_k = g + 2 < g1, has_v = g >= g0;
         if (has_k) ok = mbar_wait_all(&tl->full[0][k_slot], k_ph, abort_flag);
@@ -391,7 +401,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           if (lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
           break;
         }
-        if (g >= first && g < end) {
+        if (g >= t_begin && g < t_end) {
           if (!mbar_wait_all(&tl->p_full[i][buf], (uint32_t)(kp >> 1) & 1u, abort_flag)) {
             if (lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
             ok = false;
@@ -399,24 +409,25 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           }
           tc_fence_after();
           // O += P V: 16 keys a step, 2048 bytes of V, 8 columns of P
-          const uint64_t bd = vd + (uint64_t)(v_slot * (kApmKvBytes >> 4));
+          const uint32_t bd = vd + v_slot * (kApmKvBytes >> 4);
           if (leader) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_bf16_ts(o_col, s_col + buf * 64 + 8 * kk, bd + 128u * kk, kIdescPv, (kp | kk) ? 1u : 0u);
-            umma_commit(g + 1 < end ? &tl->o_done[i] : &tl->o_last[i]);
+              umma_bf16_ts<kUmmaDescHiSw128>(o_col, s_col + buf * 64 + 8 * kk, bd + 128u * kk, kIdescPv,
+                                             (kp | kk) ? 1u : 0u);
+            umma_commit(g + 1 < t_end ? &tl->o_done[i] : &tl->o_last[i]);
           }
           __syncwarp();
         }
-        if (g + 2 >= first && g + 2 < end) {
+        if (g + 2 >= t_begin && g + 2 < t_end) {
           tc_fence_after();
           // S = Q K^T: 16 dims a step, 32 bytes of each row
-          const uint64_t bd = kd + (uint64_t)(k_slot * (kApmKvBytes >> 4));
+          const uint32_t bd = kd + k_slot * (kApmKvBytes >> 4);
           if (leader) {
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
-              umma_bf16_ss(s_col + buf * 64, qd + (uint64_t)((kk >> 2) * (kApmHalf >> 4) + (kk & 3) * 2),
-                           bd + (uint64_t)((kk >> 2) * (kApmKvHalf >> 4) + (kk & 3) * 2), kIdescQk, kk ? 1u : 0u);
+              umma_bf16_ss<kUmmaDescHiSw128>(s_col + buf * 64, qd + (kk >> 2) * (kApmHalf >> 4) + (kk & 3) * 2,
+                                             bd + (kk >> 2) * (kApmKvHalf >> 4) + (kk & 3) * 2, kIdescQk, kk ? 1u : 0u);
             umma_commit(&tl->s_full[i][buf]);
           }
           __syncwarp();
@@ -441,20 +452,20 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       }
     }
   } else {
-    regs_inc<kApmRegsSoftmax>();
     // ------------------------------------------------------------- softmax
     const int wg = warp >> 2;  // tile
     const int r = tid & 127;   // row of the tile
+    const int row_tok = (int)(r * p.group_inv >> 16);  // its token
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + lanes + 256 + wg * 128;
-    const int first = tl->hi_max[wg] == 0 ? 0 : first_of(wg);
-    const int n = tl->hi_max[wg] == 0 ? 0 : end_of(wg) - first;  // the tile's key blocks
+    const int first_block = wg == 0 ? first[0] : first[1];
+    const int n = (wg == 0 ? end[0] : end[1]) - first_block;  // the tile's key blocks
     float m_ref = -INFINITY, l = 0.f;
     float slope2 = 0.f;
     int pos = 0;
     if (BIAS) {
-      pos = tl->pos0 + tl->tok0 + wg * tt + r / G;
-      if (valid) slope2 = p.mod.slopes[kvh * G + r % G] * 1.4426950408889634f;
+      pos = pos0 + tok0 + wg * tt + row_tok;
+      if (valid) slope2 = p.mod.slopes[kvh * G + r - row_tok * G] * 1.4426950408889634f;
     }
     bool ok = true;
 #pragma unroll 1
@@ -465,13 +476,13 @@ __global__ void __launch_bounds__(kApmThreads, 1)
         break;
       }
       tc_fence_after();
-      const int g = first + b, j0 = g * kApmBlock;
+      const int g = first_block + b, j0 = g * kApmBlock;
       float x[64];
       tmem_ld32_nowait(s_addr, x);
       tmem_ld32_nowait(s_addr + 32, x + 32);
       const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&tl->bad[g & 15]);
       const bool masked = j0 < w_lo || j0 + kApmBlock > w_hi || bad != 0;  // for some live row of the warp
-      if (j0 < tl->lo_max || j0 + kApmBlock > tl->hi_min) {
+      if (j0 < lo_max || j0 + kApmBlock > hi_min) {
         // not visible to all live rows of the CTA: V values that are not finite to zero
         const int m = g - g0;
         if (!mbar_wait_warp(&tl->full[1][m % kApmStages], (uint32_t)(m / kApmStages) & 1u, abort_flag)) {
@@ -509,20 +520,20 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           a1 = max3(a1, fabsf(x[c + 2]), fabsf(x[c + 3]));
         }
         a0 = fmaxf(a0, a1);
-        const bool small = !__any_sync(0xffffffffu, !(a0 <= p.mod.poly_max));
+        const bool small = !__any_sync(0xffffffffu, !(a0 * a0 <= p.mod.poly_max2));
         direct = !BIAS && small && !masked && p.mod.cap2 * 0.605f <= kApmBound;
         if (direct) {
           const float w = a0 * a0;
-          m_new = a0 * fmaf(fmaf(fmaf(fmaf(p.mod.poly[4], w, p.mod.poly[3]), w, p.mod.poly[2]), w, p.mod.poly[1]), w,
-                            p.mod.poly[0]);
+          m_new = a0 * fmaf(fmaf(fmaf(fmaf(p.mod.poly[4].x, w, p.mod.poly[3].x), w, p.mod.poly[2].x), w, p.mod.poly[1].x), w,
+                            p.mod.poly[0].x);
         } else if (small) {
           f32x2 pc[5];
 #pragma unroll
-          for (int k = 0; k < 5; ++k) pc[k] = pack2(p.mod.poly[k], p.mod.poly[k]);
+          for (int k = 0; k < 5; ++k) { pc[k] = pack2(p.mod.poly[k].x, p.mod.poly[k].x); asm volatile("" : "+l"(pc[k])); }
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
             const f32x2 v = pack2(x[c], x[c + 1]);
-            unpack2(mul2(v, cap_poly(mul2(v, v), pc)), x[c], x[c + 1]);
+            unpack2(mul2(v, cap_poly_r(mul2(v, v), pc)), x[c], x[c + 1]);
           }
         } else {
 #pragma unroll
@@ -584,12 +595,12 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       if (CAP && direct) {
         f32x2 pc[5];
 #pragma unroll
-        for (int k = 0; k < 5; ++k) pc[k] = pack2(p.mod.poly[k], p.mod.poly[k]);
+        for (int k = 0; k < 5; ++k) { pc[k] = pack2(p.mod.poly[k].x, p.mod.poly[k].x); asm volatile("" : "+l"(pc[k])); }
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
           const f32x2 v = pack2(x[2 * c], x[2 * c + 1]);
           float e0, e1;
-          unpack2(fma2(v, cap_poly(mul2(v, v), pc), neg2), e0, e1);
+          unpack2(fma2(v, cap_poly_r(mul2(v, v), pc), neg2), e0, e1);
           e0 = ex2(e0);
           e1 = ex2(e1);
           sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
@@ -623,66 +634,76 @@ __global__ void __launch_bounds__(kApmThreads, 1)
     tc_fence_after();
     // the output is staged where the tile's Q was: all its Q K^T are done, or
     // there were none and the load only has to have landed
-    if (n == 0 && g1 > g0) ok = mbar_wait_warp(&tl->q_full, 0, abort_flag);
+    if (n == 0 && seq >= 0) ok = mbar_wait_warp(&tl->q_full, 0, abort_flag);
     if (!ok) {
       if (lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
     } else {
-      const int seq = tl->seq, t_first = tl->t_first, q_len = tl->q_len, tok0 = tl->tok0 + wg * tt;
       const bool dead = !live || n == 0;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = dead || l == 0.f ? 0.f : 1.f / l;
       // the row's output to shared memory: 16-byte pieces, 128-byte swizzle,
       // then whole rows to global memory
       uint8_t* tile_smem = q_smem + wg * kApmTileBytes;
-      const bool poison = n > 0 && *reinterpret_cast<volatile int*>(&tl->poison) != 0;
+      auto piece = [&](int row, int d8) {  // dims 8 d8 .. 8 d8 + 7
+        return reinterpret_cast<uint4*>(tile_smem + (d8 >> 3) * kApmHalf + row * 128 + (((d8 & 7) ^ (row & 7)) << 4));
+      };
+      float o[128];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        float v[32];
         if (n > 0) {
-          tmem_ld32_nowait(o_addr + 32 * c, v);
-          tmem_wait_ld();
+          tmem_ld32_nowait(o_addr + 32 * c, o + 32 * c);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[32 * c + i] = 0.f;
         }
+      }
+      tmem_wait_ld64(o);
+      tmem_wait_ld64(o + 64);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = dead ? 0.f : v[i] * inv;
-        if (poison && live) {
-          for (int b = 0; b < n; ++b) {
-            const int j0 = (first + b) * kApmBlock;
-            if (j0 >= tl->lo_max && j0 + kApmBlock <= tl->hi_min) continue;  // not cleaned
-            for (int j = max(lo, j0); j < min(hi, j0 + kApmBlock); ++j) {
-              const long long sl = apm_slot(p, p.block_table + (size_t)seq * p.bt_stride, j);
-              if (sl < 0) continue;
-              const __nv_bfloat16* vr =
-                  p.pool + ((size_t)sl * 2 * p.n_kv_heads + p.n_kv_heads + kvh) * kHeadDim + 32 * c;
+      for (int c = 0; c < 16; ++c) {
+        uint32_t w[4];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float f = __bfloat162float(vr[i]);
-                if (!isfinite(f)) v[i] += f;
-              }
+        for (int i = 0; i < 4; ++i)
+          w[i] = dead ? 0u : pack_bf16x2(o[8 * c + 2 * i] * inv, o[8 * c + 2 * i + 1] * inv);
+        *piece(r, c) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      if (n > 0 && live && *reinterpret_cast<volatile int*>(&tl->poison) != 0) {
+        // V values that were taken out, to the rows that see them
+#pragma unroll 1
+        for (int j = lo; j < hi; ++j) {
+          const int j0 = j / kApmBlock * kApmBlock;
+          if (j0 >= lo_max && j0 + kApmBlock <= hi_min) {  // a block that was not cleaned
+            j = j0 + kApmBlock - 1;
+            continue;
+          }
+          const long long sl = apm_slot(p, p.block_table + (size_t)seq * p.bt_stride, j);
+          if (sl < 0) continue;
+          const uint4* vr = reinterpret_cast<const uint4*>(
+              p.pool + ((size_t)sl * 2 * p.n_kv_heads + p.n_kv_heads + kvh) * kHeadDim);
+#pragma unroll 1
+          for (int d8 = 0; d8 < 16; ++d8) {
+            const uint4 q = vr[d8];
+            if ((not_finite2(q.x) | not_finite2(q.y) | not_finite2(q.z) | not_finite2(q.w)) == 0) continue;
+            __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(piece(r, d8));
+            const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(vr + d8);
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              const float f = __bfloat162float(from[i]);
+              if (!isfinite(f)) at[i] = __float2bfloat16(__bfloat162float(at[i]) + f);
             }
           }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 w = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                                     pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
-          *reinterpret_cast<uint4*>(tile_smem + (c >> 1) * kApmHalf + r * 128 + ((((c & 1) * 4 + i) ^ (r & 7)) << 4)) =
-              w;
-        }
       }
       if (valid && p.lse)
-        p.lse[(size_t)(t_first + tok0 + r / G) * p.lse_stride + kvh * G + r % G] =
+        p.lse[(size_t)(t_first + tok0 + wg * tt + row_tok) * p.lse_stride + kvh * G + r - row_tok * G] =
             (dead || l == 0.f) ? -INFINITY : (m_ref == -INFINITY ? l : (m_ref + log2f(l)) * kLn2);
       __syncwarp();
-      const int r0 = (warp & 3) * 32;
-#pragma unroll 4
+      const int d8 = lane & 15, rows = min(tt, q_len - tok0 - wg * tt) * G;  // rows of the tile that exist
+      __nv_bfloat16* out = p.out + (size_t)(t_first + tok0 + wg * tt) * p.out_stride + (size_t)kvh * G * kHeadDim + d8 * 8;
+#pragma unroll 8
       for (int it = 0; it < 16; ++it) {
-        const int rr = r0 + 2 * it + (lane >> 4), ch = lane & 15;
-        const int tk = tok0 + rr / G;
-        if (seq >= 0 && rr < tt * G && tk < q_len) {
-          const uint4 w = *reinterpret_cast<const uint4*>(tile_smem + (ch >> 3) * kApmHalf + rr * 128 +
-                                                          (((ch & 7) ^ (rr & 7)) << 4));
-          *reinterpret_cast<uint4*>(p.out + (size_t)(t_first + tk) * p.out_stride +
-                                    (size_t)(kvh * G + rr % G) * kHeadDim + ch * 8) = w;
-        }
+        const int rr = (warp & 3) * 32 + 2 * it + (lane >> 4), tk = (int)(rr * p.group_inv >> 16);
+        if (seq >= 0 && rr < rows)
+          *reinterpret_cast<uint4*>(out + (size_t)tk * p.out_stride + (rr - tk * G) * kHeadDim) = *piece(rr, d8);
       }
     }
   }
@@ -774,6 +795,7 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   p.n_kv_heads = a->n_kv_heads;
   p.group = a->n_heads / a->n_kv_heads;
   p.tile_tokens = kApmRows / p.group;
+  p.group_inv = 65536u / p.group + 1;
   p.out_stride = a->out_stride;
   p.lse_stride = a->lse_stride;
   p.mod = make_score_mod(a->scale, a->softcap, a->alibi_slopes, a->window);
