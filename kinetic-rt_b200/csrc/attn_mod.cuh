@@ -18,9 +18,9 @@ struct ScoreMod {
   float cap_in;      // 2 * log2(e) * scale / cap: ex2(s * cap_in) = e^(2 x / c)
   const float* slopes;  // [n_heads] or NULL
   int window;        // 0 = none
-  // cap by polynomial while s^2 <= poly_max2: x = s * P(s^2), see cap_poly
+  // cap by polynomial while |s| <= poly_max: x = s * P(s^2), see cap_poly
   float2 poly[5];    // each coefficient twice: operands of packed multiply-adds
-  float poly_max2;   // negative: never
+  float poly_max;    // negative: never
 };
 
 inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, int window) {
@@ -35,7 +35,7 @@ inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, 
   m.window = window;
   // cap2 * tanh(u), u = a s, as an odd polynomial in s (cap_poly's coefficients times cap2 a^(2k+1));
   // left out where powers of a could leave the range of a float
-  m.poly_max2 = -1.f;
+  m.poly_max = -1.f;
   for (int k = 0; k < 5; ++k) m.poly[k] = make_float2(0.f, 0.f);
   if (softcap > 0.f) {
     static const double c[5] = {0.9999985098838806, -0.33326974511146545, 0.13257454335689545, -0.05019525811076164,
@@ -44,7 +44,7 @@ inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, 
     if (a > 1e-4 && a < 1e3 && softcap < 1e6f) {
       double f = a * m.cap2;
       for (int k = 0; k < 5; ++k, f *= a * a) m.poly[k] = make_float2((float)(c[k] * f), (float)(c[k] * f));
-      m.poly_max2 = (float)(0.7 / a * (0.7 / a));
+      m.poly_max = (float)(0.7 / a);
     }
   }
   return m;
@@ -111,12 +111,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // by at most 9.5e-8.  Scores beyond that take cap_score.  Five multiply-adds
 // and no special-function operation, of which the softmax needs all: tanh by
 // ex2 and rcp would triple them.
-__device__ __forceinline__ f32x2 cap_poly(f32x2 w, const float2* c) {
-  return fma2(fma2(fma2(fma2(pair_of(c[4]), w, pair_of(c[3])), w, pair_of(c[2])), w, pair_of(c[1])), w, pair_of(c[0]));
+__device__ __forceinline__ f32x2 cap_poly(f32x2 w, const f32x2* c) {
+  return fma2(fma2(fma2(fma2(c[4], w, c[3]), w, c[2]), w, c[1]), w, c[0]);
 }
-// The same for one value, times s: the capped score of s = sqrt(w).
-__device__ __forceinline__ float cap_at(float w, const float2* c) {
-  return sqrtf(w) * fmaf(fmaf(fmaf(fmaf(c[4].x, w, c[3].x), w, c[2].x), w, c[1].x), w, c[0].x);
+// The capped score of s, one value.
+__device__ __forceinline__ float cap_at(float s, const float2* c) {
+  const float w = s * s;
+  return s * fmaf(fmaf(fmaf(fmaf(c[4].x, w, c[3].x), w, c[2].x), w, c[1].x), w, c[0].x);
 }
 
 }  // namespace krt

@@ -85,6 +85,7 @@ struct ApmParams {
   const int32_t* kv_start;
   const int32_t* prefix_lens;
   int* status;
+  uint32_t* queue;           // [next item, CTAs that are through], zero between launches
   int num_tokens, num_seqs, bt_stride, num_blocks, tokens_per_block;
   int n_kv_heads, group, tile_tokens;  // tile_tokens = 128 / group
   uint32_t group_inv;                  // row / group = row * group_inv >> 16 for rows below 128
@@ -92,21 +93,35 @@ struct ApmParams {
   ScoreMod mod;
 };
 
+// One piece of work: a pair of tiles of one sequence and KV head.  Filled in by
+// the scheduling warp one item ahead of the others.
+struct ApmItem {
+  int seq;                // -1: there is no more work
+  int kvh;
+  int t_first, q_len;     // the sequence's first row, and its rows
+  int tok0, pos0;         // first token of the tiles; position of the sequence's first query
+  int prefix;
+  int first[2], end[2];   // key blocks of each tile, [first, end); both 0 without a live row
+  int lo_all, hi_all;     // keys that some live row sees
+  int lo_max, hi_min;     // keys that all live rows see
+};
+
 struct ApmSmemTail {
   uint64_t full[2][kApmStages];   // K, V
   uint64_t empty[2][kApmStages];
-  uint64_t q_full;
+  uint64_t item_full[2], item_empty[2];
+  uint64_t q_full, q_empty;
   uint64_t s_full[2][2];  // per tile and buffer
   uint64_t p_full[2][2];
-  uint64_t o_done[2];     // per tile: one phase per P V
-  uint64_t o_last[2];     // per tile: the last P V (two may be under way when the last P is reported)
+  uint64_t o_done[2];     // per tile: one phase per P V but an item's last
+  uint64_t o_last[2];     // per tile: an item's last P V (two may be under way when the last P is reported)
   uint64_t drain[2];      // per tile: the MMAs issued before an abort
+  ApmItem item[2];
   uint32_t tmem_base;
-  int issued[2];          // blocks of K and V requested
+  int issued[3];          // blocks of K and of V, and pairs of Q tiles, requested
   int abort;
-  int poison;             // a V value that is not finite was taken out of a partly visible block
-  int lo_min[2], hi_max[2];        // per tile, over its live rows
-  int lo_max, hi_min;              // over the CTA's live rows
+  int poison[2];          // per item: its number + 1 if a V value that is not finite was taken out of a
+                          // partly visible block
   uint32_t bad[16];       // per block (ring): pages that could not be looked up
 };
 
@@ -118,10 +133,6 @@ inline size_t apm_smem_bytes() {
 __device__ __forceinline__ void apm_fail(const ApmParams& p, ApmSmemTail* tl, int code) {
   atomicOr(p.status, code);
   *reinterpret_cast<volatile int*>(&tl->abort) = 1;
-}
-
-__device__ __forceinline__ f32x2 cap_poly_r(f32x2 w, const f32x2* c) {
-  return fma2(fma2(fma2(fma2(c[4], w, c[3]), w, c[2]), w, c[1]), w, c[0]);
 }
 
 // Exponent bits all ones in either bf16 half of w: a 1 in bit 15 or 31.
@@ -136,10 +147,111 @@ __device__ __forceinline__ long long apm_slot(const ApmParams& p, const int32_t*
   return (long long)blk * p.tokens_per_block + j % p.tokens_per_block;
 }
 
+// First position that the query at `pos` sees, apart from kv_start.
+__device__ __forceinline__ int apm_lowest(const ApmParams& p, int pos) {
+  return p.mod.window > 0 ? max(0, pos - p.mod.window + 1) : 0;
+}
+
+// Item number `index` (seq -1: there are fewer): sequences in order, the last
+// (heaviest) tokens of each first, KV heads innermost.  By a whole warp, 128
+// sequences at a time, so that their loads overlap.
+__device__ __noinline__ void apm_find(const ApmParams& p, int index, int lane, ApmItem* item) {
+  const int tt = p.tile_tokens;
+  const int kvh = index % p.n_kv_heads, target = index / p.n_kv_heads;
+  int seq = -1, t_first = 0, q_len = 0, pos0 = 0, tok0 = 0, base = 0;
+#pragma unroll 1
+  for (int s0 = 0; s0 < p.num_seqs && seq < 0; s0 += 128) {
+    int a[4], e[4], p0[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = s0 + 32 * k + lane;
+      const bool in = s < p.num_seqs;
+      a[k] = in ? p.q_start[s] : 0;
+      e[k] = in ? p.q_start[s + 1] : 0;
+      p0[k] = in ? p.q_pos0[s] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (s0 + 32 * k >= p.num_seqs) break;
+      if (a[k] < 0 || e[k] > p.num_tokens || e[k] < a[k]) atomicOr(p.status, kStatusBadBlock);
+      a[k] = max(a[k], 0);
+      e[k] = min(e[k], p.num_tokens);
+      const int n = e[k] > a[k] ? (e[k] - a[k] + 2 * tt - 1) / (2 * tt) : 0;
+      int incl = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += v;
+      }
+      const int excl = base + incl - n;
+      const uint32_t hit = __ballot_sync(0xffffffffu, target >= excl && target < excl + n);
+      if (hit != 0) {
+        const int who = __ffs(hit) - 1;
+        seq = s0 + 32 * k + who;
+        t_first = __shfl_sync(0xffffffffu, a[k], who);
+        q_len = __shfl_sync(0xffffffffu, e[k], who) - t_first;
+        pos0 = __shfl_sync(0xffffffffu, p0[k], who);
+        tok0 = (__shfl_sync(0xffffffffu, n, who) - 1 - (target - __shfl_sync(0xffffffffu, excl, who))) * 2 * tt;
+      }
+      base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  ApmItem it;
+  it.seq = seq;
+  it.kvh = kvh;
+  it.t_first = t_first;
+  it.q_len = q_len;
+  it.tok0 = tok0;
+  it.pos0 = pos0;
+  it.prefix = p.prefix_lens && seq >= 0 ? p.prefix_lens[seq] : 0;
+  it.lo_all = INT_MAX;
+  it.hi_all = 0;
+  it.lo_max = 0;
+  it.hi_min = INT_MAX;
+  const bool pos_ok = pos0 >= 0 && pos0 <= kApmMaxPos && q_len <= kApmMaxPos;
+  if (!pos_ok && lane == 0) atomicOr(p.status, kStatusBadBlock);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int lo_min = INT_MAX, hi_max = 0;  // over the tile's live rows
+    const int from = tok0 + i * tt, to = min(from + tt, q_len) - 1;  // its tokens
+    if (seq >= 0 && pos_ok && from <= to) {
+      auto highest = [&](int pos) { return min(pos0 + q_len, max(pos + 1, it.prefix)); };
+      if (p.kv_start == nullptr) {
+        // every row is live; bounds do not decrease from token to token
+        lo_min = apm_lowest(p, pos0 + from);
+        hi_max = highest(pos0 + to);
+        it.lo_max = max(it.lo_max, apm_lowest(p, pos0 + to));
+        it.hi_min = min(it.hi_min, highest(pos0 + from));
+      } else {
+        int lo_max = 0, hi_min = INT_MAX;
+        for (int tok = from + lane; tok <= to; tok += 32) {
+          const int lo = max(apm_lowest(p, pos0 + tok), p.kv_start[t_first + tok]), hi = highest(pos0 + tok);
+          if (lo >= hi) continue;
+          lo_min = min(lo_min, lo);
+          lo_max = max(lo_max, lo);
+          hi_min = min(hi_min, hi);
+          hi_max = max(hi_max, hi);
+        }
+        lo_min = __reduce_min_sync(0xffffffffu, lo_min);
+        hi_max = __reduce_max_sync(0xffffffffu, hi_max);
+        it.lo_max = max(it.lo_max, (int)__reduce_max_sync(0xffffffffu, lo_max));
+        it.hi_min = min(it.hi_min, (int)__reduce_min_sync(0xffffffffu, hi_min));
+      }
+    }
+    it.first[i] = hi_max > 0 ? lo_min / kApmBlock : 0;
+    it.end[i] = hi_max > 0 ? (hi_max + kApmBlock - 1) / kApmBlock : 0;
+    it.lo_all = min(it.lo_all, lo_min);
+    it.hi_all = max(it.hi_all, hi_max);
+  }
+  if (it.hi_all == 0) it.lo_all = 0;
+  *item = it;
+}
+
 template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kApmThreads, 1)
     paged_attention_prefill_mod_kernel(const __grid_constant__ CUtensorMap tmap_q,
-                                       const __grid_constant__ CUtensorMap tmap_kv, const ApmParams p) {
+                                       const __grid_constant__ CUtensorMap tmap_kv,
+                                       const __grid_constant__ ApmParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {  // swizzled tiles need it; the whole CTA
     if (threadIdx.x == 0) atomicOr(p.status, kStatusBadSplit);
@@ -152,7 +264,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.group, tt = p.tile_tokens;
 
-  if (warp == 8 && lane == 0) {  // (the warp that uses q_full before the others see it)
+  if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       for (int s = 0; s < kApmStages; ++s) {
         mbar_init(&tl->full[i][s], 1);
@@ -165,16 +277,15 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       mbar_init(&tl->o_done[i], 1);
       mbar_init(&tl->o_last[i], 1);
       mbar_init(&tl->drain[i], 1);
-      tl->issued[i] = 0;
-      tl->lo_min[i] = INT_MAX;
-      tl->hi_max[i] = 0;
+      mbar_init(&tl->item_full[i], 1);
+      mbar_init(&tl->item_empty[i], kApmSoftmaxWarps + 3);  // and V's producer, and both tiles' MMAs
+      tl->poison[i] = 0;
     }
     mbar_init(&tl->q_full, 1);
+    mbar_init(&tl->q_empty, 2);
     fence_mbar_init();
     tl->abort = 0;
-    tl->poison = 0;
-    tl->lo_max = 0;
-    tl->hi_min = INT_MAX;
+    tl->issued[0] = tl->issued[1] = tl->issued[2] = 0;
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_kv);
   }
@@ -184,216 +295,176 @@ __global__ void __launch_bounds__(kApmThreads, 1)
   }
   pdl_wait();  // q, the pool and the lengths come from earlier kernels
   pdl_launch_dependents();
-
-  // ---- this CTA's (sequence, pair of tiles): sequences in order, the last
-  // (heaviest) tokens of each first, KV heads innermost.  Every warp finds it
-  // by itself, 128 sequences at a time, so that their loads overlap.
-  const int kvh = (int)(blockIdx.x % (unsigned)p.n_kv_heads);
-  const int target = (int)(blockIdx.x / (unsigned)p.n_kv_heads);
-  int seq = -1, t_first = 0, q_len = 0, pos0 = 0, tok0 = 0;
-  {
-    int base = 0;
-#pragma unroll 1
-    for (int s0 = 0; s0 < p.num_seqs && seq < 0; s0 += 128) {
-      int a[4], e[4], p0[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int s = s0 + 32 * k + lane;
-        const bool in = s < p.num_seqs;
-        a[k] = in ? p.q_start[s] : 0;
-        e[k] = in ? p.q_start[s + 1] : 0;
-        p0[k] = in ? p.q_pos0[s] : 0;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (s0 + 32 * k >= p.num_seqs) break;
-        if (warp == 0 && (a[k] < 0 || e[k] > p.num_tokens || e[k] < a[k]))
-          atomicOr(p.status, kStatusBadBlock);
-        a[k] = max(a[k], 0);
-        e[k] = min(e[k], p.num_tokens);
-        const int n = e[k] > a[k] ? (e[k] - a[k] + 2 * tt - 1) / (2 * tt) : 0;
-        int incl = n;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, incl, d);
-          if (lane >= d) incl += v;
-        }
-        const int excl = base + incl - n;
-        const uint32_t hit = __ballot_sync(0xffffffffu, target >= excl && target < excl + n);
-        if (hit != 0) {
-          const int who = __ffs(hit) - 1;
-          seq = s0 + 32 * k + who;
-          t_first = __shfl_sync(0xffffffffu, a[k], who);
-          q_len = __shfl_sync(0xffffffffu, e[k], who) - t_first;
-          pos0 = __shfl_sync(0xffffffffu, p0[k], who);
-          tok0 = (__shfl_sync(0xffffffffu, n, who) - 1 - (target - __shfl_sync(0xffffffffu, excl, who))) * 2 * tt;
-        }
-        base += __shfl_sync(0xffffffffu, incl, 31);
-      }
-    }
-  }
-  __syncwarp();  // warp 8: q_full is initialised
-  if (warp == 8 && seq >= 0 && elect_one()) {
-    // the queries; keys and values follow when the blocks that are seen are known
-    mbar_arrive_expect_tx(&tl->q_full, 4u * (uint32_t)(tt * G) * 128u);
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i)
-      tma_load_4d(q_smem + i * kApmHalf, &tmap_q, &tl->q_full, 0, kvh * G, t_first + tok0 + (i >> 1) * tt, i & 1);
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tl->tmem_base;
-
-  // ---- bounds of every row, of the warp, of the tiles and of the CTA
-  int lo = 0, hi = INT_MAX;  // this row's; rows that are not live stay unmasked, their result is not used
-  bool live = false, valid = false;
-  int w_lo, w_hi;            // largest lo and smallest hi of the warp's live rows
-  int lo_max, hi_min;        // and of the CTA's
-  int first[2], end[2];      // key blocks of each tile, [first, end); both 0 without a live row
-  int lo_all, hi_all;        // keys that some live row of the CTA sees
-  {
-    const bool pos_ok = pos0 >= 0 && pos0 <= kApmMaxPos && q_len <= kApmMaxPos;
-    if (tid == 0 && !pos_ok) atomicOr(p.status, kStatusBadBlock);
-    const int prefix = p.prefix_lens && seq >= 0 ? p.prefix_lens[seq] : 0;
-    // what the query at position `at` sees, apart from kv_start: monotonous in `at`
-    auto lowest = [&](int at) { return p.mod.window > 0 ? max(0, at - p.mod.window + 1) : 0; };
-    auto highest = [&](int at) { return min(pos0 + q_len, max(at + 1, prefix)); };
-    const int r = tid & 127, tok = tok0 + (warp >> 2) * tt + (int)(r * p.group_inv >> 16);
-    valid = seq >= 0 && warp < kApmSoftmaxWarps && r < tt * G && tok < q_len;
-    if (valid && pos_ok) {
-      const int l = max(lowest(pos0 + tok), p.kv_start ? p.kv_start[t_first + tok] : 0);
-      const int h = highest(pos0 + tok);
-      live = l < h;
-      if (live) {
-        lo = l;
-        hi = h;
-      }
-    }
-    w_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0);
-    w_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);
-    int lo_min[2], hi_max[2];
-    if (p.kv_start == nullptr) {
-      // every row is live, and the tiles' first and last tokens have the extremes
-      lo_max = 0;
-      hi_min = INT_MAX;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int from = tok0 + i * tt, to = min(from + tt, q_len) - 1;
-        const bool some = pos_ok && from <= to;
-        lo_min[i] = some ? lowest(pos0 + from) : INT_MAX;
-        hi_max[i] = some ? highest(pos0 + to) : 0;
-        if (some) {
-          lo_max = lowest(pos0 + to);
-          if (hi_min == INT_MAX) hi_min = highest(pos0 + from);
-        }
-      }
-    } else {
-      const int w_lo_min = __reduce_min_sync(0xffffffffu, live ? lo : INT_MAX);
-      const int w_hi_max = __reduce_max_sync(0xffffffffu, live ? hi : 0);
-      if (warp < kApmSoftmaxWarps && lane == 0) {
-        atomicMax(&tl->lo_max, w_lo);
-        atomicMin(&tl->hi_min, w_hi);
-        atomicMin(&tl->lo_min[warp >> 2], w_lo_min);
-        atomicMax(&tl->hi_max[warp >> 2], w_hi_max);
-      }
-      __syncthreads();
-      lo_max = tl->lo_max;
-      hi_min = tl->hi_min;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        lo_min[i] = tl->lo_min[i];
-        hi_max[i] = tl->hi_max[i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      first[i] = hi_max[i] > 0 ? lo_min[i] / kApmBlock : 0;
-      end[i] = hi_max[i] > 0 ? (hi_max[i] + kApmBlock - 1) / kApmBlock : 0;
-    }
-    lo_all = min(lo_min[0], lo_min[1]);
-    hi_all = max(hi_max[0], hi_max[1]);
-  }
-  const int g0 = hi_all > 0 ? lo_all / kApmBlock : 0;
-  const int g1 = hi_all > 0 ? (hi_all + kApmBlock - 1) / kApmBlock : 0;
   volatile int* abort_flag = &tl->abort;
+  // Item k lies in slot k & 1 while it is worked on.
+  auto next_item = [&](int k) -> const ApmItem* {
+    return mbar_wait_all(&tl->item_full[k & 1], (uint32_t)(k >> 1) & 1u, abort_flag) ? &tl->item[k & 1] : nullptr;
+  };
+  auto release_item = [&](int k) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tl->item_empty[k & 1]);
+  };
 
-  if (warp >= kApmSoftmaxWarps) {
-    if ((warp == 8 || warp == 11) && g1 > g0) {
-      // ---------------------------------------------- producers of K and of V
-      // One lane issues all of a block's boxes, from values that the warp has
-      // in common (boxes issued by several lanes take about 100 cycles each).
-      const int kv = warp == 8 ? 0 : 1;
-      const bool leader = elect_one();
-      const uint64_t pol = make_l2_policy_evict_last();  // K and V are read again by other tiles
-      const int outside = p.num_blocks * p.tokens_per_block;  // a box there reads zeros
-      const int32_t* table = p.block_table + (size_t)seq * p.bt_stride;
+  if (warp == 8 || warp == 11) {
+    // ------------------------------------------------ producers of K and of V
+    // One lane issues all of a block's boxes, from values that the warp has in
+    // common (boxes issued by several lanes take about 100 cycles each).  K's
+    // producer also finds the work: when an item's last K is under way it takes
+    // the next from the queue, so that nothing of this is waited for.
+    const int kv = warp == 8 ? 0 : 1;
+    const bool leader = elect_one();
+    const uint64_t pol = make_l2_policy_evict_last();  // K and V are read again by other tiles
+    const int outside = p.num_blocks * p.tokens_per_block;  // a box there reads zeros
+    uint8_t* ring = kv ? v_smem : k_smem;
+    int slot = 0, count = 0, q_count = 0;  // count: blocks requested so far
+    uint32_t ph = 0;
+    bool ok = true;
+    ApmItem it = {};
+    if (kv == 0) apm_find(p, (int)blockIdx.x, lane, &it);
+#pragma unroll 1
+    for (int k = 0; ok; ++k) {
+      if (kv == 0) {
+        if (k > 1 && !mbar_wait_all(&tl->item_empty[k & 1], (uint32_t)((k >> 1) - 1) & 1u, abort_flag)) {
+          if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
+          break;
+        }
+        if (leader) {
+          tl->item[k & 1] = it;
+          mbar_arrive(&tl->item_full[k & 1]);
+        }
+        __syncwarp();
+      } else {
+        const ApmItem* at = next_item(k);
+        if (at == nullptr) {
+          if (lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
+          break;
+        }
+        it = *at;
+        release_item(k);
+      }
+      if (it.seq < 0) {
+        if (kv == 0 && leader) {
+          // this CTA takes no more; the last one to say so leaves the queue empty for the next launch
+          __threadfence();
+          if (atomicAdd(p.queue + 1, 1u) + 1 == gridDim.x) {
+            p.queue[0] = 0u;
+            p.queue[1] = 0u;
+          }
+        }
+        break;
+      }
+      const int g0 = it.lo_all / kApmBlock, g1 = (it.hi_all + kApmBlock - 1) / kApmBlock;
+      const int32_t* table = p.block_table + (size_t)it.seq * p.bt_stride;
       // pool token of this lane's page of block g (lanes 0-3), -1 where the lookup failed
       auto look_up = [&](int g) {
         const int j = g * kApmBlock + (lane & 3) * kApmPage;
         int v = outside;
-        if (g < g1 && j < hi_all && j + kApmPage > lo_all) v = (int)apm_slot(p, table, j);
+        if (g < g1 && j < it.hi_all && j + kApmPage > it.lo_all) v = (int)apm_slot(p, table, j);
         return v;
       };
-      uint8_t* ring = kv ? v_smem : k_smem;
-      int slot = 0, pool_tok = look_up(g0), next_tok = look_up(g0 + 1);
-      uint32_t ph = 0;
+      int pool_tok = look_up(g0), next_tok = look_up(g0 + 1);
+      if (kv == 0 && g1 > g0) {
+        if (q_count > 0 && !mbar_wait_all(&tl->q_empty, (uint32_t)(q_count - 1) & 1u, abort_flag)) {
+          if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
+          break;
+        }
+        ++q_count;
+        if (leader) {
+          mbar_arrive_expect_tx(&tl->q_full, 4u * (uint32_t)(tt * G) * 128u);
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i)
+            tma_load_4d(q_smem + i * kApmHalf, &tmap_q, &tl->q_full, 0, it.kvh * G,
+                        it.t_first + it.tok0 + (i >> 1) * tt, i & 1);
+          tl->issued[2] = q_count;
+        }
+        __syncwarp();
+      }
 #pragma unroll 1
       for (int g = g0; g < g1; ++g) {
         const uint32_t bad = __ballot_sync(0xffffffffu, pool_tok < 0) & 15u;
         if (pool_tok < 0) pool_tok = outside;
         int page[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) page[k] = __shfl_sync(0xffffffffu, pool_tok, k);
+        for (int c = 0; c < 4; ++c) page[c] = __shfl_sync(0xffffffffu, pool_tok, c);
         pool_tok = next_tok;
         next_tok = look_up(g + 2);  // two blocks ahead: the lookup is not waited for
-        if (g - g0 >= kApmStages && !mbar_wait_all(&tl->empty[kv][slot], ph ^ 1u, abort_flag)) {
+        if (count >= kApmStages && !mbar_wait_all(&tl->empty[kv][slot], ph ^ 1u, abort_flag)) {
           if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
+          ok = false;
           break;
         }
         if (leader) {
           if (kv == 0) {
-            *reinterpret_cast<volatile uint32_t*>(&tl->bad[g & 15]) = bad;
+            *reinterpret_cast<volatile uint32_t*>(&tl->bad[count & 15]) = bad;
             if (bad != 0) atomicOr(p.status, kStatusBadBlock);
           }
           mbar_arrive_expect_tx(&tl->full[kv][slot], kApmKvBytes);
           uint8_t* dst = ring + (size_t)slot * kApmKvBytes;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            tma_load_5d(dst + k * 2048, &tmap_kv, &tl->full[kv][slot], 0, page[k], 0, kv, kvh, pol);
-            tma_load_5d(dst + k * 2048 + kApmKvHalf, &tmap_kv, &tl->full[kv][slot], 0, page[k], 1, kv, kvh, pol);
+          for (int c = 0; c < 4; ++c) {
+            tma_load_5d(dst + c * 2048, &tmap_kv, &tl->full[kv][slot], 0, page[c], 0, kv, it.kvh, pol);
+            tma_load_5d(dst + c * 2048 + kApmKvHalf, &tmap_kv, &tl->full[kv][slot], 0, page[c], 1, kv, it.kvh, pol);
           }
-          tl->issued[kv] = g - g0 + 1;
+          tl->issued[kv] = count + 1;
         }
         __syncwarp();
+        ++count;
         if (++slot == kApmStages) {
           slot = 0;
           ph ^= 1u;
         }
       }
-    } else if (warp >= 9 && warp <= 10 && g1 > g0) {
-      // ---------------------------------------------------------- UMMA issue
-      // One warp per tile; the whole warp walks the loop, one lane issues.  Step
-      // g: P V of block g, then Q K^T of block g + 2 into the buffer that this
-      // frees.  MMAs of one thread run in the order of their issue.
-      constexpr uint32_t kIdescQk = umma_idesc_bf16(128, 64);
-      constexpr uint32_t kIdescPv = umma_idesc_bf16(128, 128) | kUmmaBMnMajor;
-      const int i = warp - 9;
-      const bool leader = elect_one();
-      const uint32_t qd = umma_desc_lo(smem_u32(q_smem)) + i * (kApmTileBytes >> 4);
-      const uint32_t kd = umma_desc_lo(smem_u32(k_smem));
-      const uint32_t vd = umma_desc_lo_mn(smem_u32(v_smem), kApmKvHalf);
-      // (a tile without a live row has no blocks in any step)
-      const int t_end = i == 0 ? end[0] : end[1], t_begin = t_end == 0 ? g1 : (i == 0 ? first[0] : first[1]);
-      const uint32_t s_col = tmem + i * 128, o_col = tmem + 256 + i * 128;
-      int k_slot = 0, v_slot = 0;
-      uint32_t k_ph = 0, v_ph = 0;
-      bool ok = mbar_wait_all(&tl->q_full, 0, abort_flag);
-      if (!ok && lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
+      if (kv == 0 && ok) {
+        uint32_t taken = 0;
+        if (lane == 0) taken = atomicAdd(p.queue, 1u);
+        apm_find(p, (int)(gridDim.x + __shfl_sync(0xffffffffu, taken, 0)), lane, &it);
+      }
+    }
+  } else if (warp > 8) {
+    // ------------------------------------------------------------ UMMA issue
+    // One warp per tile; the whole warp walks the loop, one lane issues.  Step
+    // g: P V of block g, then Q K^T of block g + 2 into the buffer that this
+    // frees.  MMAs of one thread run in the order of their issue.
+    constexpr uint32_t kIdescQk = umma_idesc_bf16(128, 64);
+    constexpr uint32_t kIdescPv = umma_idesc_bf16(128, 128) | kUmmaBMnMajor;
+    const int i = warp - 9;
+    const bool leader = elect_one();
+    const uint32_t qd = umma_desc_lo(smem_u32(q_smem)) + i * (kApmTileBytes >> 4);
+    const uint32_t kd = umma_desc_lo(smem_u32(k_smem));
+    const uint32_t vd = umma_desc_lo_mn(smem_u32(v_smem), kApmKvHalf);
+    const uint32_t s_col = tmem + i * 128, o_col = tmem + 256 + i * 128;
+    int k_slot = 0, v_slot = 0, q_count = 0;
+    uint32_t k_ph = 0, v_ph = 0;
+    int done = 0;  // the tile's blocks of earlier items
+    bool ok = true;
 #pragma unroll 1
-      for (int g = g0 - 2; g < g1 && ok; ++g) {
-        const int kp = g - t_begin;  // the tile's how-manieth block; its buffer is kp & 1
-        const uint32_t buf = (uint32_t)kp & 1u;
+    for (int k = 0; ok; ++k) {
+      const ApmItem* at = next_item(k);
+      if (at == nullptr) {
+        if (lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
+        ok = false;
+        break;
+      }
+      const int seq = at->seq, g0 = at->lo_all / kApmBlock, g1 = (at->hi_all + kApmBlock - 1) / kApmBlock;
+      // (a tile without a live row has no blocks in any step)
+      const int t_end = at->end[i], t_begin = t_end == 0 ? g1 : at->first[i];
+      release_item(k);
+      if (seq < 0) break;
+      if (g1 <= g0) continue;
+      if (!mbar_wait_all(&tl->q_full, (uint32_t)q_count & 1u, abort_flag)) {
+        if (lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
+        ok = false;
+        break;
+      }
+      ++q_count;
+#pragma unroll 1
+      for (int g = g0 - 2; g < g1; ++g) {
+        const int b = g - t_begin;             // the item's how-manieth block of the tile
+        const uint32_t n = (uint32_t)(done + b);  // of all items; its buffer is n & 1
         const bool has_k = g + 2 < g1, has_v = g >= g0;
         if (has_k) ok = mbar_wait_all(&tl->full[0][k_slot], k_ph, abort_flag);
         if (has_v && ok) ok = mbar_wait_all(&tl->full[1][v_slot], v_ph, abort_flag);
@@ -402,7 +473,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           break;
         }
         if (g >= t_begin && g < t_end) {
-          if (!mbar_wait_all(&tl->p_full[i][buf], (uint32_t)(kp >> 1) & 1u, abort_flag)) {
+          if (!mbar_wait_all(&tl->p_full[i][n & 1], (n >> 1) & 1u, abort_flag)) {
             if (lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
             ok = false;
             break;
@@ -413,8 +484,8 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           if (leader) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_bf16_ts<kUmmaDescHiSw128>(o_col, s_col + buf * 64 + 8 * kk, bd + 128u * kk, kIdescPv,
-                                             (kp | kk) ? 1u : 0u);
+              umma_bf16_ts<kUmmaDescHiSw128>(o_col, s_col + (n & 1) * 64 + 8 * kk, bd + 128u * kk, kIdescPv,
+                                             (b | kk) ? 1u : 0u);
             umma_commit(g + 1 < t_end ? &tl->o_done[i] : &tl->o_last[i]);
           }
           __syncwarp();
@@ -426,15 +497,16 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           if (leader) {
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
-              umma_bf16_ss<kUmmaDescHiSw128>(s_col + buf * 64, qd + (kk >> 2) * (kApmHalf >> 4) + (kk & 3) * 2,
+              umma_bf16_ss<kUmmaDescHiSw128>(s_col + (n & 1) * 64, qd + (kk >> 2) * (kApmHalf >> 4) + (kk & 3) * 2,
                                              bd + (kk >> 2) * (kApmKvHalf >> 4) + (kk & 3) * 2, kIdescQk, kk ? 1u : 0u);
-            umma_commit(&tl->s_full[i][buf]);
+            umma_commit(&tl->s_full[i][n & 1]);
           }
           __syncwarp();
         }
         if (leader) {
           if (has_v) umma_commit(&tl->empty[1][v_slot]);
           if (has_k) umma_commit(&tl->empty[0][k_slot]);
+          if (g + 3 == g1) umma_commit(&tl->q_empty);  // the item's last Q K^T
         }
         __syncwarp();
         if (has_v && ++v_slot == kApmStages) {
@@ -446,272 +518,282 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           k_ph ^= 1u;
         }
       }
-      if (!ok && leader) {  // what was issued reads shared memory and writes TMEM until it is done
-        umma_commit(&tl->drain[i]);
-        mbar_wait(&tl->drain[i], 0, nullptr);
-      }
+      done += t_end - (t_end == 0 ? 0 : t_begin);
+    }
+    if (!ok && leader) {  // what was issued reads shared memory and writes TMEM until it is done
+      umma_commit(&tl->drain[i]);
+      mbar_wait(&tl->drain[i], 0, nullptr);
     }
   } else {
-    // ------------------------------------------------------------- softmax
+    // --------------------------------------------------------------- softmax
     const int wg = warp >> 2;  // tile
     const int r = tid & 127;   // row of the tile
     const int row_tok = (int)(r * p.group_inv >> 16);  // its token
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + lanes + 256 + wg * 128;
-    const int first_block = wg == 0 ? first[0] : first[1];
-    const int n = (wg == 0 ? end[0] : end[1]) - first_block;  // the tile's key blocks
-    float m_ref = -INFINITY, l = 0.f;
-    float slope2 = 0.f;
-    int pos = 0;
-    if (BIAS) {
-      pos = pos0 + tok0 + wg * tt + row_tok;
-      if (valid) slope2 = p.mod.slopes[kvh * G + r - row_tok * G] * 1.4426950408889634f;
-    }
+    int done = 0, blocks = 0, last = 0, partial_pv = 0;  // of earlier items: the tile's blocks, the CTA's, o_last's and
+                                                          // o_done's phases
     bool ok = true;
 #pragma unroll 1
-    for (int b = 0; b < n; ++b) {
-      const uint32_t s_addr = tmem + lanes + wg * 128 + (b & 1) * 64;
-      if (!mbar_wait_all(&tl->s_full[wg][b & 1], (uint32_t)(b >> 1) & 1u, abort_flag)) {
+    for (int k = 0; ok; ++k) {
+      const ApmItem* at = next_item(k);
+      if (at == nullptr) {
         ok = false;
         break;
       }
-      tc_fence_after();
-      const int g = first_block + b, j0 = g * kApmBlock;
-      float x[64];
-      tmem_ld32_nowait(s_addr, x);
-      tmem_ld32_nowait(s_addr + 32, x + 32);
-      const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&tl->bad[g & 15]);
-      const bool masked = j0 < w_lo || j0 + kApmBlock > w_hi || bad != 0;  // for some live row of the warp
-      if (j0 < lo_max || j0 + kApmBlock > hi_min) {
-        // not visible to all live rows of the CTA: V values that are not finite to zero
-        const int m = g - g0;
-        if (!mbar_wait_warp(&tl->full[1][m % kApmStages], (uint32_t)(m / kApmStages) & 1u, abort_flag)) {
+      if (at->seq < 0) break;
+      // ---- this row's bounds, and the warp's
+      const int first = at->first[wg], n = at->end[wg] - first;  // the tile's key blocks
+      int lo = 0, hi = INT_MAX;  // rows that are not live stay unmasked, their result is not used
+      bool live = false;
+      const int tok = at->tok0 + wg * tt + row_tok, pos = at->pos0 + tok;
+      const bool valid = r < tt * G && tok < at->q_len;
+      if (valid && n > 0) {
+        const int l = max(apm_lowest(p, pos), p.kv_start ? p.kv_start[at->t_first + tok] : 0);
+        const int h = min(at->pos0 + at->q_len, max(pos + 1, at->prefix));
+        live = l < h;
+        if (live) {
+          lo = l;
+          hi = h;
+        }
+      }
+      const int w_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0);        // keys that all live rows of the
+      const int w_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);  // warp see
+      const int g0 = at->lo_all / kApmBlock;
+      float m_ref = -INFINITY, l = 0.f;
+      float slope2 = 0.f;
+      if (BIAS && valid) slope2 = p.mod.slopes[at->kvh * G + r - row_tok * G] * 1.4426950408889634f;
+#pragma unroll 1
+      for (int b = 0; b < n; ++b) {
+        const uint32_t nb = (uint32_t)(done + b);
+        const uint32_t s_addr = tmem + lanes + wg * 128 + (nb & 1) * 64;
+        if (!mbar_wait_all(&tl->s_full[wg][nb & 1], (nb >> 1) & 1u, abort_flag)) {
           ok = false;
           break;
         }
-        uint4* v = reinterpret_cast<uint4*>(v_smem + (size_t)(m % kApmStages) * kApmKvBytes);
-#pragma unroll 4
-        for (int i = 0; i < 8; ++i) {
-          uint4 q = v[i * 128 + r];
-          if ((not_finite2(q.x) | not_finite2(q.y) | not_finite2(q.z) | not_finite2(q.w)) != 0) {
-            *reinterpret_cast<volatile int*>(&tl->poison) = 1;
-            __threadfence_block();
-            auto clean = [](uint32_t w) {
-              const uint32_t f = not_finite2(w);
-              return w & ((f & 0x8000u ? 0u : 0xFFFFu) | (f & 0x80000000u ? 0u : 0xFFFF0000u));
-            };
-            v[i * 128 + r] = make_uint4(clean(q.x), clean(q.y), clean(q.z), clean(q.w));
-          }
-        }
-        // the tensor core sees the values written; P V starts when all four
-        // warps have reported their P, so after all of the block is clean
-        fence_proxy_async_smem();
-      }
-      tmem_wait_ld();
-      // ---- modifications (base 2).  `direct`: scores stay q . k, and the scale
-      // or the cap's polynomial enters in the exponent
-      bool direct = !CAP && !BIAS;
-      float m_new = -INFINITY;
-      if (CAP) {
-        float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          a0 = max3(a0, fabsf(x[c]), fabsf(x[c + 1]));
-          a1 = max3(a1, fabsf(x[c + 2]), fabsf(x[c + 3]));
-        }
-        a0 = fmaxf(a0, a1);
-        const bool small = !__any_sync(0xffffffffu, !(a0 * a0 <= p.mod.poly_max2));
-        direct = !BIAS && small && !masked && p.mod.cap2 * 0.605f <= kApmBound;
-        if (direct) {
-          const float w = a0 * a0;
-          m_new = a0 * fmaf(fmaf(fmaf(fmaf(p.mod.poly[4].x, w, p.mod.poly[3].x), w, p.mod.poly[2].x), w, p.mod.poly[1].x), w,
-                            p.mod.poly[0].x);
-        } else if (small) {
-          f32x2 pc[5];
-#pragma unroll
-          for (int k = 0; k < 5; ++k) { pc[k] = pack2(p.mod.poly[k].x, p.mod.poly[k].x); asm volatile("" : "+l"(pc[k])); }
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const f32x2 v = pack2(x[c], x[c + 1]);
-            unpack2(mul2(v, cap_poly_r(mul2(v, v), pc)), x[c], x[c + 1]);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 64; ++c) x[c] = cap_score(x[c], p.mod.cap_in, p.mod.cap2);
-        }
-      }
-      if (BIAS) {
-        const float d0 = (float)(j0 - pos);
-#pragma unroll
-        for (int c = 0; c < 64; ++c) x[c] = fmaf(-slope2, fabsf(d0 + (float)c), CAP ? x[c] : x[c] * p.mod.mul);
-      }
-      if (masked) {
-        const int v0 = lo - j0, v1 = hi - j0;
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < v0 || c >= v1 || ((bad >> (c / kApmPage)) & 1u)) x[c] = -INFINITY;
-      }
-      if (!(CAP && direct)) {
-        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          mx[0] = max3(mx[0], x[c], x[c + 1]);
-          mx[1] = max3(mx[1], x[c + 2], x[c + 3]);
-        }
-        m_new = fmaxf(mx[0], mx[1]);
-        if (direct) m_new *= p.mod.mul;
-      }
-      // ---- the row's reference
-      const bool grow = m_new > m_ref + kApmLazy;  // also from -inf
-      if (__any_sync(0xffffffffu, grow)) {
-        const float f = grow ? ex2(m_ref - m_new) : 1.f;
-        if (grow) m_ref = m_new;
-        l *= f;
-        if (b > 0) {
-          // the previous block's P V may still run (the one before it is done: S
-          // of this block was computed after it)
-          if (!mbar_wait_warp(&tl->o_done[wg], (uint32_t)(b - 1) & 1u, abort_flag)) {
+        tc_fence_after();
+        const int g = first + b, j0 = g * kApmBlock;
+        float x[64];
+        tmem_ld32_nowait(s_addr, x);
+        tmem_ld32_nowait(s_addr + 32, x + 32);
+        const int m = blocks + g - g0;  // of the CTA's blocks
+        const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&tl->bad[m & 15]);
+        const bool masked = j0 < w_lo || j0 + kApmBlock > w_hi || bad != 0;  // for some live row of the warp
+        if (j0 < at->lo_max || j0 + kApmBlock > at->hi_min) {
+          // not visible to all live rows of the CTA: V values that are not finite to zero
+          if (!mbar_wait_warp(&tl->full[1][m % kApmStages], (uint32_t)(m / kApmStages) & 1u, abort_flag)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float v[32];
-            uint32_t w[32];
-            tmem_ld32_nowait(o_addr + 32 * c, v);
-            tmem_wait_ld();
+          uint4* v = reinterpret_cast<uint4*>(v_smem + (size_t)(m % kApmStages) * kApmKvBytes);
+#pragma unroll 4
+          for (int i = 0; i < 8; ++i) {
+            uint4 q = v[i * 128 + r];
+            if ((not_finite2(q.x) | not_finite2(q.y) | not_finite2(q.z) | not_finite2(q.w)) != 0) {
+              *reinterpret_cast<volatile int*>(&tl->poison[k & 1]) = k + 1;
+              __threadfence_block();
+              auto clean = [](uint32_t w) {
+                const uint32_t f = not_finite2(w);
+                return w & ((f & 0x8000u ? 0u : 0xFFFFu) | (f & 0x80000000u ? 0u : 0xFFFF0000u));
+              };
+              v[i * 128 + r] = make_uint4(clean(q.x), clean(q.y), clean(q.z), clean(q.w));
+            }
+          }
+          // the tensor core sees the values written; P V starts when all four
+          // warps have reported their P, so after all of the block is clean
+          fence_proxy_async_smem();
+        }
+        tmem_wait_ld64(x);
+        // ---- modifications (base 2).  `direct`: scores stay q . k, and the scale
+        // or the cap's polynomial enters in the exponent
+        bool direct = !CAP && !BIAS;
+        float m_new = -INFINITY;
+        f32x2 pc[5];  // the polynomial, kept in registers: as constants they slow the multiply-adds down
+        if (CAP) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * f);
-            tmem_st32(o_addr + 32 * c, w);
+          for (int c = 0; c < 5; ++c) {
+            pc[c] = pair_of(p.mod.poly[c]);
+            asm volatile("" : "+l"(pc[c]));
+          }
+          float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            a0 = max3(a0, fabsf(x[c]), fabsf(x[c + 1]));
+            a1 = max3(a1, fabsf(x[c + 2]), fabsf(x[c + 3]));
+          }
+          a0 = fmaxf(a0, a1);
+          const bool small = !__any_sync(0xffffffffu, !(a0 <= p.mod.poly_max));
+          direct = !BIAS && small && !masked && p.mod.cap2 * 0.605f <= kApmBound;
+          if (direct) {
+            m_new = cap_at(a0, p.mod.poly);  // a reference no lower than the maximum
+          } else if (small) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+              const f32x2 v = pack2(x[c], x[c + 1]);
+              unpack2(mul2(v, cap_poly(mul2(v, v), pc)), x[c], x[c + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 64; ++c) x[c] = cap_score(x[c], p.mod.cap_in, p.mod.cap2);
+          }
+        }
+        if (BIAS) {
+          const float d0 = (float)(j0 - pos);
+#pragma unroll
+          for (int c = 0; c < 64; ++c) x[c] = fmaf(-slope2, fabsf(d0 + (float)c), CAP ? x[c] : x[c] * p.mod.mul);
+        }
+        if (masked) {
+          const int v0 = lo - j0, v1 = hi - j0;
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c < v0 || c >= v1 || ((bad >> (c / kApmPage)) & 1u)) x[c] = -INFINITY;
+        }
+        if (!(CAP && direct)) {
+          float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            mx[0] = max3(mx[0], x[c], x[c + 1]);
+            mx[1] = max3(mx[1], x[c + 2], x[c + 3]);
+          }
+          m_new = fmaxf(mx[0], mx[1]);
+          if (direct) m_new *= p.mod.mul;
+        }
+        // ---- the row's reference
+        const bool grow = m_new > m_ref + kApmLazy;  // also from -inf
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? ex2(m_ref - m_new) : 1.f;
+          if (grow) m_ref = m_new;
+          l *= f;
+          if (b > 0) {
+            // the previous block's P V may still run (the one before it is done: S
+            // of this block was computed after it)
+            if (!mbar_wait_warp(&tl->o_done[wg], (uint32_t)(partial_pv + b - 1) & 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float v[32];
+              uint32_t w[32];
+              tmem_ld32_nowait(o_addr + 32 * c, v);
+              tmem_wait_ld32(v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * f);
+              tmem_st32(o_addr + 32 * c, w);
+            }
+          }
+        }
+        // ---- weights: 2^(x - reference), packed to bf16 as they come
+        const float neg = m_ref == -INFINITY ? 0.f : -m_ref;  // nothing seen yet: weights 0, NaN stays NaN
+        const f32x2 neg2 = pack2(neg, neg);
+        f32x2 sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+        uint32_t pk[32];
+        if (CAP && direct) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const f32x2 v = pack2(x[2 * c], x[2 * c + 1]);
+            float e0, e1;
+            unpack2(fma2(v, cap_poly(mul2(v, v), pc), neg2), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
+            pk[c] = pack_bf16x2(e0, e1);
+          }
+        } else {
+          const f32x2 mul_2 = pack2(p.mod.mul, p.mod.mul);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            f32x2 y = pack2(x[2 * c], x[2 * c + 1]);
+            y = (CAP || BIAS) ? add2(y, neg2) : fma2(y, mul_2, neg2);
+            float e0, e1;
+            unpack2(y, e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
+            pk[c] = pack_bf16x2(e0, e1);
+          }
+        }
+        tmem_st32(s_addr, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tl->p_full[wg][nb & 1]);
+        float s0, s1;
+        unpack2(add2(sum2[0], sum2[1]), s0, s1);
+        l += s0 + s1;
+      }
+      if (!ok) break;
+      // ------------------------------------------------------------ the rows out
+      if (n > 0) {
+        if (!mbar_wait_all(&tl->o_last[wg], (uint32_t)last & 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        ++last;
+        partial_pv += n - 1;
+      }
+      const int t = at->t_first + tok, head = at->kvh * G + r - row_tok * G;
+      __nv_bfloat16* out = p.out + (size_t)t * p.out_stride + (size_t)head * kHeadDim;
+      const float inv = !live || l == 0.f ? 0.f : 1.f / l;
+      // a row's 256 bytes are written by its thread; the L2 joins the pieces
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float o[64];
+        if (n > 0) {
+          tmem_ld32_nowait(o_addr + 64 * c, o);
+          tmem_ld32_nowait(o_addr + 64 * c + 32, o + 32);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) o[i] = 0.f;
+        }
+        tmem_wait_ld64(o);
+        if (valid) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = live ? pack_bf16x2(o[8 * i + 2 * e] * inv, o[8 * i + 2 * e + 1] * inv) : 0u;
+            *reinterpret_cast<uint4*>(out + 64 * c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
       }
-      // ---- weights: 2^(x - reference), packed to bf16 as they come
-      const float neg = m_ref == -INFINITY ? 0.f : -m_ref;  // nothing seen yet: weights 0, NaN stays NaN
-      const f32x2 neg2 = pack2(neg, neg);
-      f32x2 sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-      uint32_t pk[32];
-      if (CAP && direct) {
-        f32x2 pc[5];
-#pragma unroll
-        for (int k = 0; k < 5; ++k) { pc[k] = pack2(p.mod.poly[k].x, p.mod.poly[k].x); asm volatile("" : "+l"(pc[k])); }
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const f32x2 v = pack2(x[2 * c], x[2 * c + 1]);
-          float e0, e1;
-          unpack2(fma2(v, cap_poly_r(mul2(v, v), pc), neg2), e0, e1);
-          e0 = ex2(e0);
-          e1 = ex2(e1);
-          sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
-          pk[c] = pack_bf16x2(e0, e1);
-        }
-      } else {
-        const f32x2 mul_2 = pack2(p.mod.mul, p.mod.mul);
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          f32x2 y = pack2(x[2 * c], x[2 * c + 1]);
-          y = (CAP || BIAS) ? add2(y, neg2) : fma2(y, mul_2, neg2);
-          float e0, e1;
-          unpack2(y, e0, e1);
-          e0 = ex2(e0);
-          e1 = ex2(e1);
-          sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
-          pk[c] = pack_bf16x2(e0, e1);
-        }
-      }
-      tmem_st32(s_addr, pk);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tl->p_full[wg][b & 1]);
-      float s0, s1;
-      unpack2(add2(sum2[0], sum2[1]), s0, s1);
-      l += s0 + s1;
-    }
-    // ------------------------------------------------------------ epilogue
-    if (n > 0 && ok) ok = mbar_wait_warp(&tl->o_last[wg], 0, abort_flag);
-    tc_fence_after();
-    // the output is staged where the tile's Q was: all its Q K^T are done, or
-    // there were none and the load only has to have landed
-    if (n == 0 && seq >= 0) ok = mbar_wait_warp(&tl->q_full, 0, abort_flag);
-    if (!ok) {
-      if (lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
-    } else {
-      const bool dead = !live || n == 0;
-      const float inv = dead || l == 0.f ? 0.f : 1.f / l;
-      // the row's output to shared memory: 16-byte pieces, 128-byte swizzle,
-      // then whole rows to global memory
-      uint8_t* tile_smem = q_smem + wg * kApmTileBytes;
-      auto piece = [&](int row, int d8) {  // dims 8 d8 .. 8 d8 + 7
-        return reinterpret_cast<uint4*>(tile_smem + (d8 >> 3) * kApmHalf + row * 128 + (((d8 & 7) ^ (row & 7)) << 4));
-      };
-      float o[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (n > 0) {
-          tmem_ld32_nowait(o_addr + 32 * c, o + 32 * c);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[32 * c + i] = 0.f;
-        }
-      }
-      tmem_wait_ld64(o);
-      tmem_wait_ld64(o + 64);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = dead ? 0u : pack_bf16x2(o[8 * c + 2 * i] * inv, o[8 * c + 2 * i + 1] * inv);
-        *piece(r, c) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      if (n > 0 && live && *reinterpret_cast<volatile int*>(&tl->poison) != 0) {
+      // (O is read: the next item's first P, which its P V waits for, comes later)
+      if (live && *reinterpret_cast<volatile int*>(&tl->poison[k & 1]) == k + 1) {
         // V values that were taken out, to the rows that see them
 #pragma unroll 1
         for (int j = lo; j < hi; ++j) {
           const int j0 = j / kApmBlock * kApmBlock;
-          if (j0 >= lo_max && j0 + kApmBlock <= hi_min) {  // a block that was not cleaned
+          if (j0 >= at->lo_max && j0 + kApmBlock <= at->hi_min) {  // a block that was not cleaned
             j = j0 + kApmBlock - 1;
             continue;
           }
-          const long long sl = apm_slot(p, p.block_table + (size_t)seq * p.bt_stride, j);
+          const long long sl = apm_slot(p, p.block_table + (size_t)at->seq * p.bt_stride, j);
           if (sl < 0) continue;
-          const uint4* vr = reinterpret_cast<const uint4*>(
-              p.pool + ((size_t)sl * 2 * p.n_kv_heads + p.n_kv_heads + kvh) * kHeadDim);
+          const __nv_bfloat16* v = p.pool + ((size_t)sl * 2 * p.n_kv_heads + p.n_kv_heads + at->kvh) * kHeadDim;
 #pragma unroll 1
-          for (int d8 = 0; d8 < 16; ++d8) {
-            const uint4 q = vr[d8];
-            if ((not_finite2(q.x) | not_finite2(q.y) | not_finite2(q.z) | not_finite2(q.w)) == 0) continue;
-            __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(piece(r, d8));
-            const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(vr + d8);
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-              const float f = __bfloat162float(from[i]);
-              if (!isfinite(f)) at[i] = __float2bfloat16(__bfloat162float(at[i]) + f);
-            }
+          for (int i = 0; i < kHeadDim; ++i) {
+            const float f = __bfloat162float(v[i]);
+            if (!isfinite(f)) out[i] = __float2bfloat16(__bfloat162float(out[i]) + f);
           }
         }
       }
       if (valid && p.lse)
-        p.lse[(size_t)(t_first + tok0 + wg * tt + row_tok) * p.lse_stride + kvh * G + r - row_tok * G] =
-            (dead || l == 0.f) ? -INFINITY : (m_ref == -INFINITY ? l : (m_ref + log2f(l)) * kLn2);
-      __syncwarp();
-      const int d8 = lane & 15, rows = min(tt, q_len - tok0 - wg * tt) * G;  // rows of the tile that exist
-      __nv_bfloat16* out = p.out + (size_t)(t_first + tok0 + wg * tt) * p.out_stride + (size_t)kvh * G * kHeadDim + d8 * 8;
-#pragma unroll 8
-      for (int it = 0; it < 16; ++it) {
-        const int rr = (warp & 3) * 32 + 2 * it + (lane >> 4), tk = (int)(rr * p.group_inv >> 16);
-        if (seq >= 0 && rr < rows)
-          *reinterpret_cast<uint4*>(out + (size_t)tk * p.out_stride + (rr - tk * G) * kHeadDim) = *piece(rr, d8);
-      }
+        p.lse[(size_t)t * p.lse_stride + head] =
+            !live || l == 0.f ? -INFINITY : (m_ref == -INFINITY ? l : (m_ref + log2f(l)) * kLn2);
+      done += n;
+      blocks += (at->hi_all + kApmBlock - 1) / kApmBlock - g0;
+      release_item(k);
     }
+    if (!ok && lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
   }
   tc_fence_before();
   __syncthreads();
   if (tl->abort && tid == 0) {
     // loads still in flight land (bounded waits) before the CTA's memory goes
-    mbar_wait(&tl->q_full, 0, nullptr);
+    if (tl->issued[2] > 0) mbar_wait(&tl->q_full, (uint32_t)(tl->issued[2] - 1) & 1u, nullptr);
     for (int kv = 0; kv < 2; ++kv)
       for (int m = max(0, tl->issued[kv] - kApmStages); m < tl->issued[kv]; ++m)
         mbar_wait(&tl->full[kv][m % kApmStages], (uint32_t)(m / kApmStages) & 1u, nullptr);
@@ -740,7 +822,7 @@ extern "C" size_t krt_paged_attention_prefill_mod_workspace_size(int32_t num_tok
   if (num_tokens <= 0 || num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 ||
       max_kv_len <= 0)
     return 0;
-  return kWsHeaderBytes;
+  return kWsHeaderBytes;  // status word, and the queue behind it
 }
 
 extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention_mod_args* a, void* stream) {
@@ -787,6 +869,7 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   p.kv_start = a->kv_start;
   p.prefix_lens = a->prefix_lens;
   p.status = static_cast<int*>(a->workspace);
+  p.queue = reinterpret_cast<uint32_t*>(static_cast<char*>(a->workspace) + 256);
   p.num_tokens = a->num_tokens;
   p.num_seqs = a->num_seqs;
   p.bt_stride = a->block_table_stride;
@@ -814,7 +897,8 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_error(e, name);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * a->n_kv_heads), 1, 1);
+  const long long items = tiles * a->n_kv_heads, sms = device_sm_count();
+  cfg.gridDim = dim3((unsigned)(items < sms ? items : sms), 1, 1);
   cfg.blockDim = dim3(kApmThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
