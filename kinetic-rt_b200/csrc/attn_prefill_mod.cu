@@ -64,13 +64,14 @@ namespace krt {
 constexpr int kApmRows = 128;    // rows of a tile (TMEM lanes)
 constexpr int kApmBlock = 64;    // keys per block
 constexpr int kApmPage = 16;     // tokens per TMA box
-constexpr int kApmStages = 5;    // of K, and of V
+constexpr int kApmStages = 4;    // of K, and of V
 constexpr int kApmSoftmaxWarps = 8;
 constexpr int kApmThreads = 384;
 constexpr uint32_t kApmTileBytes = 32768;  // Q tile: 128 rows x 128 dims bf16, two [128 x 128 B] halves
 constexpr uint32_t kApmHalf = 16384;
 constexpr uint32_t kApmKvBytes = 16384;    // K or V block: 64 tokens x 128 dims, two [64 x 128 B] halves
 constexpr uint32_t kApmKvHalf = 8192;
+constexpr uint32_t kApmOutBytes = 16384;   // 64 columns of a tile's output
 constexpr float kApmLazy = 8.f;   // growth of a row's maximum (base 2) that is left unscaled
 constexpr float kApmBound = 50.f; // largest reference (base 2) that may lie above the row's maximum
 constexpr int kApmMaxPos = 1 << 30;
@@ -127,7 +128,7 @@ struct ApmSmemTail {
 
 // (no room to round the base up: the kernel checks that it is 1024-byte aligned)
 inline size_t apm_smem_bytes() {
-  return (size_t)2 * kApmTileBytes + (size_t)2 * kApmStages * kApmKvBytes + sizeof(ApmSmemTail);
+  return (size_t)2 * kApmTileBytes + (size_t)2 * kApmStages * kApmKvBytes + 2 * kApmOutBytes + sizeof(ApmSmemTail);
 }
 
 __device__ __forceinline__ void apm_fail(const ApmParams& p, ApmSmemTail* tl, int code) {
@@ -155,7 +156,7 @@ __device__ __forceinline__ int apm_lowest(const ApmParams& p, int pos) {
 // Item number `index` (seq -1: there are fewer): sequences in order, the last
 // (heaviest) tokens of each first, KV heads innermost.  By a whole warp, 128
 // sequences at a time, so that their loads overlap.
-__device__ __noinline__ void apm_find(const ApmParams& p, int index, int lane, ApmItem* item) {
+__device__ __forceinline__ ApmItem apm_find(const ApmParams& p, int index, int lane) {
   const int tt = p.tile_tokens;
   const int kvh = index % p.n_kv_heads, target = index / p.n_kv_heads;
   int seq = -1, t_first = 0, q_len = 0, pos0 = 0, tok0 = 0, base = 0;
@@ -244,7 +245,7 @@ __device__ __noinline__ void apm_find(const ApmParams& p, int index, int lane, A
     it.hi_all = max(it.hi_all, hi_max);
   }
   if (it.hi_all == 0) it.lo_all = 0;
-  *item = it;
+  return it;
 }
 
 template <bool CAP, bool BIAS>
@@ -260,7 +261,8 @@ __global__ void __launch_bounds__(kApmThreads, 1)
   uint8_t* q_smem = smem;
   uint8_t* k_smem = smem + 2 * kApmTileBytes;
   uint8_t* v_smem = k_smem + kApmStages * kApmKvBytes;
-  ApmSmemTail* tl = reinterpret_cast<ApmSmemTail*>(v_smem + kApmStages * kApmKvBytes);
+  uint8_t* out_smem = v_smem + kApmStages * kApmKvBytes;
+  ApmSmemTail* tl = reinterpret_cast<ApmSmemTail*>(out_smem + 2 * kApmOutBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.group, tt = p.tile_tokens;
 
@@ -323,11 +325,16 @@ __global__ void __launch_bounds__(kApmThreads, 1)
     int slot = 0, count = 0, q_count = 0;  // count: blocks requested so far
     uint32_t ph = 0;
     bool ok = true;
-    ApmItem it = {};
-    if (kv == 0) apm_find(p, (int)blockIdx.x, lane, &it);
 #pragma unroll 1
     for (int k = 0; ok; ++k) {
+      ApmItem it;
       if (kv == 0) {
+        uint32_t index = blockIdx.x;
+        if (k > 0) {
+          if (lane == 0) index = gridDim.x + atomicAdd(p.queue, 1u);
+          index = __shfl_sync(0xffffffffu, index, 0);
+        }
+        it = apm_find(p, (int)index, lane);
         if (k > 1 && !mbar_wait_all(&tl->item_empty[k & 1], (uint32_t)((k >> 1) - 1) & 1u, abort_flag)) {
           if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
           break;
@@ -417,11 +424,6 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           slot = 0;
           ph ^= 1u;
         }
-      }
-      if (kv == 0 && ok) {
-        uint32_t taken = 0;
-        if (lane == 0) taken = atomicAdd(p.queue, 1u);
-        apm_find(p, (int)(gridDim.x + __shfl_sync(0xffffffffu, taken, 0)), lane, &it);
       }
     }
   } else if (warp > 8) {
@@ -643,10 +645,18 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           for (int c = 0; c < 64; ++c) x[c] = fmaf(-slope2, fabsf(d0 + (float)c), CAP ? x[c] : x[c] * p.mod.mul);
         }
         if (masked) {
-          const int v0 = lo - j0, v1 = hi - j0;
+          // visible keys of the block as bits
+          const int v0 = min(max(lo - j0, 0), 64), v1 = min(max(hi - j0, 0), 64);
+          unsigned long long seen = v0 < v1 ? (~0ull >> (64 - (v1 - v0))) << v0 : 0ull;
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (c < v0 || c >= v1 || ((bad >> (c / kApmPage)) & 1u)) x[c] = -INFINITY;
+          for (int c = 0; c < 4; ++c)
+            if ((bad >> c) & 1u) seen &= ~(0xFFFFull << (16 * c));
+          const uint32_t seen0 = (uint32_t)seen, seen1 = (uint32_t)(seen >> 32);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            x[c] = (seen0 >> c) & 1u ? x[c] : -INFINITY;
+            x[32 + c] = (seen1 >> c) & 1u ? x[32 + c] : -INFINITY;
+          }
         }
         if (!(CAP && direct)) {
           float mx[2] = {-INFINITY, -INFINITY};
@@ -735,10 +745,15 @@ __global__ void __launch_bounds__(kApmThreads, 1)
         partial_pv += n - 1;
       }
       const int t = at->t_first + tok, head = at->kvh * G + r - row_tok * G;
-      __nv_bfloat16* out = p.out + (size_t)t * p.out_stride + (size_t)head * kHeadDim;
       const float inv = !live || l == 0.f ? 0.f : 1.f / l;
-      // a row's 256 bytes are written by its thread; the L2 joins the pieces
-#pragma unroll
+      // Through shared memory, 64 columns at a time (16-byte pieces, 128-byte
+      // swizzle), then whole rows: a row written by its thread alone would take
+      // a memory transaction for every 16 bytes.
+      uint8_t* stage = out_smem + wg * kApmOutBytes;
+      const int rows = min(tt, at->q_len - at->tok0 - wg * tt) * G;  // rows of the tile that exist
+      __nv_bfloat16* tile_out = p.out + (size_t)(at->t_first + at->tok0 + wg * tt) * p.out_stride +
+                                (size_t)at->kvh * G * kHeadDim + (lane & 7) * 8;
+#pragma unroll 1
       for (int c = 0; c < 2; ++c) {
         float o[64];
         if (n > 0) {
@@ -749,20 +764,29 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           for (int i = 0; i < 64; ++i) o[i] = 0.f;
         }
         tmem_wait_ld64(o);
-        if (valid) {
+        __syncwarp();  // the warp's rows of the first 64 columns are read
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t w[4];
+        for (int i = 0; i < 8; ++i) {
+          uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = live ? pack_bf16x2(o[8 * i + 2 * e] * inv, o[8 * i + 2 * e + 1] * inv) : 0u;
-            *reinterpret_cast<uint4*>(out + 64 * c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int e = 0; e < 4; ++e)
+            w[e] = live ? pack_bf16x2(o[8 * i + 2 * e] * inv, o[8 * i + 2 * e + 1] * inv) : 0u;
+          *reinterpret_cast<uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = (warp & 3) * 32 + 4 * i + (lane >> 3), tk = (int)(rr * p.group_inv >> 16);
+          if (rr < rows)
+            *reinterpret_cast<uint4*>(tile_out + (size_t)tk * p.out_stride + (rr - tk * G) * kHeadDim + 64 * c) =
+                *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
         }
       }
       // (O is read: the next item's first P, which its P V waits for, comes later)
+      __syncwarp();  // (the row may have been written by other lanes)
       if (live && *reinterpret_cast<volatile int*>(&tl->poison[k & 1]) == k + 1) {
         // V values that were taken out, to the rows that see them
+        __nv_bfloat16* out = p.out + (size_t)t * p.out_stride + (size_t)head * kHeadDim;
 #pragma unroll 1
         for (int j = lo; j < hi; ++j) {
           const int j0 = j / kApmBlock * kApmBlock;
