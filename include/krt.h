@@ -380,7 +380,11 @@ KRT_API int krt_paged_attention_prefill(const krt_paged_prefill_attention_args* 
  * above; any number of query heads per KV head up to 16; the pool holds
  * fewer than 2^31 - 16 tokens.  scale 0 = 1 / sqrt(head_dim); scale, softcap and
  * window must not be negative.  Workspaces are zero-filled once when
- * allocated; calls that may overlap on the GPU need workspaces of their own.
+ * allocated (and again after a status word with a timeout bit); calls that
+ * may overlap on the GPU need workspaces of their own.  A workspace made for
+ * the most sequences and the longest max_seq_len, passed whole, serves every
+ * smaller call of the same heads and window after one another, captured ones
+ * too.
  * ---------------------------------------------------------------------- */
 
 /* One query token per sequence, at position p = seq_lens[s] - 1 (its K/V are

@@ -8,19 +8,23 @@
 //
 // Every visible K/V byte is read once, so the kernel is bound by HBM; the
 // invisible ones (before the window or the document) are not read.  Grid
-// (sequence, KV head, split of the visible 16-token chunks); four warps take
-// the CTA's chunks in turn, each with its own ring of three 8 KB stages (one
-// 5-D TMA box = K and V of 16 tokens of one KV head, 128-byte swizzled);
-// Q K^T and P V on mma.sync m16n8k16 with the group's query heads in the rows
-// (about 4 FLOP a byte: the tensor rate does not matter), statistics and sums
-// in fp32; P is rounded to bf16 for P V (relative 2^-9, as V is).  Warps merge
-// in shared memory, splits in the workspace by the last CTA to finish, in
-// split order, so results do not depend on which CTA that is.
+// (sequence, KV head, split of the visible 16-token chunks); four or eight
+// warps take the CTA's chunks in turn, each with its own ring of three 8 KB
+// stages (one 5-D TMA box = K and V of 16 tokens of one KV head, 128-byte
+// swizzled; 192 KB under way per SM); Q K^T and P V on mma.sync m16n8k16 with
+// the group's query heads in the rows (about 4 FLOP a byte: the tensor rate
+// does not matter), statistics and sums in fp32; P is rounded to bf16 for P V
+// (relative 2^-9, as V is).  Warps merge in shared memory, splits in the
+// workspace by the last CTA to finish, in split order, so results do not
+// depend on which CTA that is.  Measured: 128 sequences of 4224 tokens, 8 KV
+// heads (2.2 GB) in 321 us = 6.9 TB/s; one sequence of 4224 tokens 11.1 us in
+// a graph, of which 5 are a CTA's start, its two merges and the launch.
 //
 // V rows of tokens that are not visible are set to zero in shared memory
 // before P V: their weight is 0, and 0 * inf or 0 * NaN from a cache slot
 // nothing was written to would spoil the row.  Only the first and last chunk
 // of the visible range hold such tokens.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -36,13 +40,11 @@
 
 namespace krt {
 
-constexpr int kAdmWarps = 4;
-constexpr int kAdmThreads = kAdmWarps * 32;
 constexpr int kAdmStages = 3;               // per warp
 constexpr int kAdmChunk = 16;               // tokens per TMA box
 constexpr uint32_t kAdmStageBytes = 8192;   // K and V of 16 tokens, one KV head
 constexpr int kAdmMaxGroup = 16;            // query heads per KV head
-constexpr int kAdmRowFloats = 2 + kHeadDim; // max, sum, 128 outputs
+constexpr int kAdmRowFloats = 4 + kHeadDim; // max, sum, (two unused), 128 outputs
 constexpr int kAdmMaxCps = 512;             // 16-token chunks per CTA at most
 
 struct AdmParams {
@@ -53,7 +55,7 @@ struct AdmParams {
   const int32_t* seq_lens;
   const int32_t* kv_start;   // [num_seqs] or NULL
   float* part;               // [num_seqs][n_kv_heads][max_splits][group][kAdmRowFloats]
-  uint32_t* counters;        // [num_seqs][n_kv_heads]
+  uint32_t* counters_end;    // counter of (sequence, KV head) i at -1 - i
   int* status;
   int bt_stride, num_blocks, tokens_per_block;
   int n_kv_heads, group;
@@ -63,14 +65,16 @@ struct AdmParams {
   ScoreMod mod;
 };
 
+template <int WARPS>
 struct AdmSmemTail {
-  uint64_t full[kAdmWarps][kAdmStages];
+  uint64_t full[WARPS][kAdmStages];
   int tok[kAdmMaxCps];  // first pool token of each of the CTA's chunks, -1 when the lookup failed
   int last;
 };
 
-inline size_t adm_smem_bytes() {
-  return 1024 + (size_t)kAdmWarps * kAdmStages * kAdmStageBytes + sizeof(AdmSmemTail);
+template <int WARPS>
+constexpr size_t adm_smem_bytes() {
+  return 1024 + (size_t)WARPS * kAdmStages * kAdmStageBytes + sizeof(AdmSmemTail<WARPS>);
 }
 
 // One merged row: 8 output values (and, by the thread of the first 8, the lse).
@@ -84,12 +88,13 @@ __device__ __forceinline__ void adm_write_row(const AdmParams& p, int b, int hea
     p.lse[(size_t)b * p.lse_stride + head] = L == 0.f ? -INFINITY : (M == -INFINITY ? L : (M + log2f(L)) * kLn2);
 }
 
-template <bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kAdmThreads, 2)
+template <int WARPS, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
     paged_attention_decode_mod_kernel(const __grid_constant__ CUtensorMap tmap_kv, const AdmParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  AdmSmemTail* tl = reinterpret_cast<AdmSmemTail*>(smem + (size_t)kAdmWarps * kAdmStages * kAdmStageBytes);
+  constexpr int kAdmWarps = WARPS, kAdmThreads = 32 * WARPS;
+  auto* tl = reinterpret_cast<AdmSmemTail<WARPS>*>(smem + (size_t)kAdmWarps * kAdmStages * kAdmStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int b = blockIdx.x, kvh = blockIdx.y, z = blockIdx.z;
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(kAdmThreads, 2)
     l_r[rr] += __shfl_xor_sync(0xffffffffu, l_r[rr], 2);
   }
 
-  // ---- merge the four warps: rows [warp][row][max, sum, 128 outputs] in the
+  // ---- merge the warps: rows [warp][row][max, sum, 128 outputs] in the
   // (now idle) stage buffers
   __syncthreads();
   float* wrow = reinterpret_cast<float*>(smem);
@@ -317,8 +322,7 @@ __global__ void __launch_bounds__(kAdmThreads, 2)
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      dst[2 + 8 * j + 2 * t4] = o[j][2 * rr];
-      dst[2 + 8 * j + 2 * t4 + 1] = o[j][2 * rr + 1];
+      *reinterpret_cast<float2*>(dst + 4 + 8 * j + 2 * t4) = make_float2(o[j][2 * rr], o[j][2 * rr + 1]);
     }
   }
   __syncthreads();
@@ -337,7 +341,7 @@ __global__ void __launch_bounds__(kAdmThreads, 2)
       const float f = M == -INFINITY ? 1.f : ex2(src[0] - M);
       L += f * src[1];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += f * src[2 + d0 + i];
+      for (int i = 0; i < 8; ++i) acc[i] += f * src[4 + d0 + i];
     }
     if (single) {
       adm_write_row(p, b, kvh * G + row, d0, acc, M, L);
@@ -347,8 +351,8 @@ __global__ void __launch_bounds__(kAdmThreads, 2)
         dst[0] = M;
         dst[1] = L;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dst[2 + d0 + i] = acc[i];
+      *reinterpret_cast<float4*>(dst + 4 + d0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(dst + 8 + d0) = make_float4(acc[4], acc[5], acc[6], acc[7]);
     }
   }
   if (single) return;
@@ -357,7 +361,7 @@ __global__ void __launch_bounds__(kAdmThreads, 2)
   __threadfence();  // this CTA's partial is visible GPU-wide before the count
   __syncthreads();
   if (threadIdx.x == 0) {
-    uint32_t* ctr = p.counters + (size_t)b * p.n_kv_heads + kvh;
+    uint32_t* ctr = p.counters_end - 1 - ((size_t)b * p.n_kv_heads + kvh);
     const uint32_t prev = atomicAdd(ctr, 1u);
     const bool last = prev + 1 == (uint32_t)splits;
     if (last) *ctr = 0u;  // ready for the next call
@@ -369,24 +373,57 @@ __global__ void __launch_bounds__(kAdmThreads, 2)
   const float* base = p.part + ((size_t)b * p.n_kv_heads + kvh) * p.max_splits * (size_t)G * kAdmRowFloats;
   for (int idx = threadIdx.x; idx < G * 16; idx += kAdmThreads) {
     const int row = idx >> 4, d0 = (idx & 15) * 8;
-    float M = -INFINITY;
-    for (int zz = 0; zz < splits; ++zz) M = fmaxf(M, __ldcg(base + ((size_t)zz * G + row) * kAdmRowFloats));
-    float L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int zz = 0; zz < splits; ++zz) {
-      const float* src = base + ((size_t)zz * G + row) * kAdmRowFloats;
-      const float f = M == -INFINITY ? 1.f : ex2(__ldcg(src) - M);
-      L += f * __ldcg(src + 1);
+    // splits in groups whose loads are all under way together: each round
+    // trip to the L2 is about a third of a short call's whole time
+    float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int z0 = 0; z0 < splits; z0 += 8) {
+      float m[8], ls[8];
+      float4 lo4[8], hi4[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += f * __ldcg(src + 2 + d0 + i);
+      for (int k = 0; k < 8; ++k) {
+        const bool in = z0 + k < splits;
+        const float* src = base + ((size_t)(in ? z0 + k : z0) * G + row) * kAdmRowFloats;
+        m[k] = in ? __ldcg(src) : -INFINITY;
+        ls[k] = in ? __ldcg(src + 1) : 0.f;
+        lo4[k] = __ldcg(reinterpret_cast<const float4*>(src + 4 + d0));
+        hi4[k] = __ldcg(reinterpret_cast<const float4*>(src + 8 + d0));
+      }
+      float mx = M;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, m[k]);
+      const float mu = mx == -INFINITY ? 0.f : mx;  // nothing seen: factors 0 of zeros, NaN stays NaN
+      const float keep = M == mx ? 1.f : ex2(M - mu);
+      M = mx;
+      L *= keep;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] *= keep;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (z0 + k >= splits) break;
+        const float f = m[k] == mx ? 1.f : ex2(m[k] - mu);
+        L += f * ls[k];
+        acc[0] += f * lo4[k].x;
+        acc[1] += f * lo4[k].y;
+        acc[2] += f * lo4[k].z;
+        acc[3] += f * lo4[k].w;
+        acc[4] += f * hi4[k].x;
+        acc[5] += f * hi4[k].y;
+        acc[6] += f * hi4[k].z;
+        acc[7] += f * hi4[k].w;
+      }
     }
     adm_write_row(p, b, kvh * G + row, d0, acc, M, L);
   }
 }
 
 typedef void (*AdmKernel)(const CUtensorMap, const AdmParams);
+template <int WARPS>
 AdmKernel adm_kernel(bool cap, bool bias) {
-  if (cap) return bias ? paged_attention_decode_mod_kernel<true, true> : paged_attention_decode_mod_kernel<true, false>;
-  return bias ? paged_attention_decode_mod_kernel<false, true> : paged_attention_decode_mod_kernel<false, false>;
+  if (cap)
+    return bias ? paged_attention_decode_mod_kernel<WARPS, true, true>
+                : paged_attention_decode_mod_kernel<WARPS, true, false>;
+  return bias ? paged_attention_decode_mod_kernel<WARPS, false, true>
+              : paged_attention_decode_mod_kernel<WARPS, false, false>;
 }
 
 }  // namespace krt
@@ -405,17 +442,29 @@ int adm_max_chunks(int max_seq_len, int window) {
   return (int)(win < all ? win : all);
 }
 
-// Chunks per CTA: the rule of the plain decode attention (at least 16, about
-// one and a half waves of two CTAs per SM, equal pieces).
-int adm_chunks_per_split(int num_seqs, int n_kv_heads, int max_chunks) {
-  const long long slots = (long long)device_sm_count() * 2;
-  const long long pairs = (long long)num_seqs * n_kv_heads;
-  long long cps = (2 * pairs * max_chunks + 3 * slots - 1) / (3 * slots);
-  if (cps < 16) cps = 16;
-  if (cps > max_chunks) cps = max_chunks;
-  if (cps > kAdmMaxCps) cps = kAdmMaxCps;
-  const long long splits = (max_chunks + cps - 1) / cps;
-  return (int)((max_chunks + splits - 1) / splits);
+// CTAs per (sequence, KV head): as many as fill the SMs once, but at most
+// sqrt(chunks) / 2 (the merge grows with their number as the scan shrinks),
+// and at least so many that none scans more than kAdmMaxCps chunks.  More,
+// smaller pieces lose: every CTA starts its pipeline, merges its warps and
+// leaves an fp32 partial.  Measured (us), pairs x chunks, this rule against
+// two CTAs per SM and more: 256 x 65 25.6 : 31.0, 160 x 63 17.5 : 25.6,
+// 128 x 128 26.0 : 31.7, 8 x 512 14.7 : 17.1 (37 splits 26.8),
+// 8 x 264 11.1 : 17.5, 24 x 4096 of ragged lengths 132 : 133 to 139.
+int adm_splits(long long pairs, int max_chunks) {
+  const int deepest = (max_chunks + kAdmMaxCps - 1) / kAdmMaxCps;
+  const long long fill = device_sm_count() / pairs;
+  const int most = (int)(std::sqrt((double)max_chunks) / 2);
+  return std::max(deepest, (int)std::min<long long>(fill, most));
+}
+
+// fp32 partial rows of the largest call of at most that many pairs and chunks
+// (a row of every query head per split), so that a workspace made for the
+// largest batch serves smaller ones, which have more splits each.
+size_t adm_part_bytes(long long pairs, int group, int max_chunks) {
+  const long long deepest = (max_chunks + kAdmMaxCps - 1) / kAdmMaxCps;
+  const long long most = std::max(1, (int)(std::sqrt((double)max_chunks) / 2));
+  const long long parts = std::max(pairs * deepest, std::min<long long>(device_sm_count(), pairs * most));
+  return (size_t)parts * group * kAdmRowFloats * 4;
 }
 
 }  // namespace
@@ -424,11 +473,9 @@ extern "C" size_t krt_paged_attention_mod_workspace_size(int32_t num_seqs, int32
                                                          int32_t max_seq_len, int32_t window) {
   if (num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || max_seq_len <= 0 || window < 0 || n_heads % n_kv_heads != 0)
     return 0;
-  const int max_chunks = adm_max_chunks(max_seq_len, window);
-  const int cps = adm_chunks_per_split(num_seqs, n_kv_heads, max_chunks);
-  const size_t max_splits = (max_chunks + cps - 1) / cps;
-  const size_t counters = ((size_t)num_seqs * n_kv_heads * 4 + 255) & ~size_t(255);
-  return kWsHeaderBytes + counters + (size_t)num_seqs * n_heads * max_splits * kAdmRowFloats * 4;
+  const long long pairs = (long long)num_seqs * n_kv_heads;
+  const size_t counters = ((size_t)pairs * 4 + 255) & ~size_t(255);
+  return kWsHeaderBytes + adm_part_bytes(pairs, n_heads / n_kv_heads, adm_max_chunks(max_seq_len, window)) + counters;
 }
 
 extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args* a, void* stream) {
@@ -475,9 +522,10 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   p.kv_start = a->kv_start;
   char* ws = static_cast<char*>(a->workspace);
   p.status = reinterpret_cast<int*>(ws);
-  p.counters = reinterpret_cast<uint32_t*>(ws + kWsHeaderBytes);
-  const size_t counters = ((size_t)a->num_seqs * a->n_kv_heads * 4 + 255) & ~size_t(255);
-  p.part = reinterpret_cast<float*>(ws + kWsHeaderBytes + counters);
+  // partials from the front, counters from the end: calls of other sizes on
+  // the same workspace never leave a partial where a counter is expected at 0
+  p.part = reinterpret_cast<float*>(ws + kWsHeaderBytes);
+  p.counters_end = reinterpret_cast<uint32_t*>(ws + (a->workspace_bytes & ~size_t(3)));
   p.bt_stride = a->block_table_stride;
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
@@ -487,20 +535,30 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   p.out_stride = a->out_stride;
   p.lse_stride = a->lse_stride;
   p.max_len = a->max_seq_len;
-  p.chunks_per_split = adm_chunks_per_split(a->num_seqs, a->n_kv_heads, max_chunks);
+  const long long pairs = (long long)a->num_seqs * a->n_kv_heads;
+  const int splits = adm_splits(pairs, max_chunks);
+  p.chunks_per_split = (max_chunks + splits - 1) / splits;
   p.max_splits = (max_chunks + p.chunks_per_split - 1) / p.chunks_per_split;
   if (p.max_splits > 65535) return set_error(KRT_ERR_UNSUPPORTED, "%s: max_seq_len is too long", name);
   p.mod = make_score_mod(a->scale, a->softcap, a->alibi_slopes, a->window);
   CUtensorMap tmap;
   int rc = make_tmap_pool_kv16(&tmap, a->kv_pool, a->num_blocks, a->tokens_per_block, a->n_kv_heads, true);
   if (rc) return rc;
-  AdmKernel kern = adm_kernel(a->softcap > 0.f, a->alibi_slopes != nullptr);
-  const size_t smem = adm_smem_bytes();
+  // Eight warps and one CTA per SM, unless the CTAs are one to two per SM:
+  // then four warps, so that all are resident at once.  Measured (us), eight :
+  // four: 100 CTAs x 264 chunks 39.7 : 45.1, 75 x 125 16.9 : 23.1,
+  // 64 x 33 11.1 : 12.6; 160 x 63 23.2 : 17.5, 256 x 65 28.4 : 25.6;
+  // 320 x 128 61.6 : 68.5, 320 x 264 117 : 136, 1024 x 264 325 : 322.
+  const long long ctas = pairs * p.max_splits;
+  const bool eight = ctas <= device_sm_count() || ctas > 2 * device_sm_count();
+  AdmKernel kern = eight ? adm_kernel<8>(a->softcap > 0.f, a->alibi_slopes != nullptr)
+                         : adm_kernel<4>(a->softcap > 0.f, a->alibi_slopes != nullptr);
+  const size_t smem = eight ? adm_smem_bytes<8>() : adm_smem_bytes<4>();
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_error(e, name);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a->num_seqs, (unsigned)a->n_kv_heads, (unsigned)p.max_splits);
-  cfg.blockDim = dim3(kAdmThreads, 1, 1);
+  cfg.blockDim = dim3(eight ? 256 : 128, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];

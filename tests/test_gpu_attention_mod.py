@@ -385,3 +385,27 @@ def test_decode_is_the_prompts_last_row(torch_cuda):
     _, _, tol, tol_lse = orc.paged_attention_mod(p.q, p.pool, p.table, p.rows(), 8, 2, 16, 25.0, 60,
                                                  np.float32(slopes_of(8)))
     assert (np.abs(got - one) <= 2 * tol).all() and (np.abs(lse - lse1) <= 2 * tol_lse).all()
+
+
+@pytest.mark.parametrize("seqs,ctx,H,K", [(1, 700, 4, 1), (2, 1024, 8, 2), (5, 3000, 4, 2), (160, 40, 1, 1),
+                                          (310, 33, 2, 1)])
+def test_decode_sizes_share_a_workspace(torch_cuda, seqs, ctx, H, K):
+    """One workspace, made for a larger batch of other heads' shape, serves calls with many and with no splits."""
+    from python.kinetic_rt import _lib
+    ws = torch_cuda.zeros(_lib.attention_mod_workspace_bytes(512, 8, 2, 4096), dtype=torch_cuda.uint8, device="cuda")
+    rng = np.random.Generator(np.random.PCG64(77))
+    lens = rng.integers(0, ctx + 1, seqs)
+    lens[0] = ctx
+    for n, L, h, k in ((seqs, lens, H, K), (3, [2000, 1, 900], 8, 2), (seqs, lens, H, K)):
+        case = Case(torch_cuda, list(map(int, L)), n_heads=h, n_kv_heads=k)
+        a = case.args()
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        case.launch(a)
+        rc, bits = _lib.read_status(ws)
+        assert rc == 0 and bits == 0
+        got, got_lse = case.result()
+        ref, lse, tol, tol_lse = orc.paged_attention_mod(case.q, case.pool, case.table, case.rows(), h, k, case.tpb)
+        assert (np.abs(got - ref) <= tol).all()
+        seen = ~np.isneginf(lse)
+        assert (np.isneginf(got_lse) == ~seen).all()
+        assert (np.abs(got_lse[seen] - lse[seen]) <= np.broadcast_to(tol_lse, lse.shape)[seen]).all()
