@@ -7,15 +7,25 @@
 // dims R .. 127 pass through.  q goes to q_out, k and v to the slot of the
 // token's cache index (token layout [K | V][kv_head][128] bf16).
 //
-// The kernel reads and writes every element once and is bound by HBM.  A CTA
-// takes a few tokens: its threads first compute each token's R / 2 cosines and
-// sines into shared memory, shared by all heads.  The angle is taken in fp64
-// turns (p * inv_freq / 2 pi) and reduced to its fraction before the fp32
-// sine: at position 10^6 an fp32 angle would be off by 0.06.  This costs R / 2
-// fp64 products a token, against R * heads products, and saves the table that
-// limits the position.  Then unit u of a head is two 8-element vectors that a
-// thread loads, rotates and stores (16-byte accesses): the two partners of a
-// half-split rotation, or two vectors of interleaved pairs.
+// The kernel reads and writes every element once and is bound by HBM.  A warp
+// takes a token (a CTA of eight warps when there are few tokens): its threads
+// ask for their first vectors, then compute the token's R / 2 cosines and
+// sines into shared memory while those are under way; all heads share them.
+// The angle is taken in fp64 turns (p * inv_freq / 2 pi) and reduced to its
+// fraction before the fp32 sine: at position 10^6 an fp32 angle would be off
+// by 0.06.  This costs R / 2 fp64 products a token, against R * heads products,
+// and saves the table that limits the position.  Unit u of a head is two
+// 8-element vectors that a thread loads, rotates and stores (16-byte
+// accesses): the two partners of a half-split rotation, or two vectors of
+// interleaved pairs.
+//
+// Measured: 16384 tokens of 32 + 8 heads (bf16, 403 MB) in 69 us = 5.9 TB/s;
+// 32 k tokens of 8 + 1 heads (fp32 in, 250 MB) in 47 us = 5.3 TB/s: with ten
+// heads the angles are a third of a warp's time on its token.  More warps
+// matter more than vectors per thread: two fp32 units per thread (two CTAs per
+// SM fewer) take 52 us, four bf16 units 72 us.  A warp per token instead of a
+// CTA for four tokens with a barrier after the angles: 74 to 69 and 60 to 47.
+// 64 tokens take 3.0 us in a graph.
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -30,7 +40,6 @@
 namespace krt {
 
 constexpr int kRaThreads = 256;
-constexpr int kRaMaxTokens = 4;  // tokens per CTA at most
 constexpr int kRaUnits = 8;      // two-vector units per head
 
 struct RaParams {
@@ -46,24 +55,39 @@ struct RaParams {
   long long q_stride, k_stride, v_stride, q_out_stride;
   int num_tokens, n_heads, n_kv_heads, rotary_dim, interleaved;
   int num_seqs, bt_stride, num_blocks, tokens_per_block;
-  int tokens_per_cta;
   float factor;
 };
 
-__device__ __forceinline__ void ra_load8(const float* src, float* x) {
-  const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-__device__ __forceinline__ void ra_load8(const __nv_bfloat16* src, float* x) {
-  const uint4 v = *reinterpret_cast<const uint4*>(src);
-  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(p[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+// Eight elements as they lie in memory (read once: marked to leave the caches
+// first), and as fp32.
+template <typename T>
+struct RaVec;
+template <>
+struct RaVec<float> {
+  static constexpr int kBatch = 1;  // units a thread has under way
+  float4 lo, hi;
+  __device__ __forceinline__ void load(const float* src) {
+    lo = __ldcs(reinterpret_cast<const float4*>(src));
+    hi = __ldcs(reinterpret_cast<const float4*>(src) + 1);
   }
-}
+  __device__ __forceinline__ void get(float* x) const {
+    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+  }
+};
+template <>
+struct RaVec<__nv_bfloat16> {
+  static constexpr int kBatch = 2;
+  uint4 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* src) { v = __ldcs(reinterpret_cast<const uint4*>(src)); }
+  __device__ __forceinline__ void get(float* x) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
 __device__ __forceinline__ float ra_load1(const float* src) { return *src; }
 __device__ __forceinline__ float ra_load1(const __nv_bfloat16* src) { return __bfloat162float(*src); }
 
@@ -72,125 +96,147 @@ __device__ __forceinline__ void ra_store8(__nv_bfloat16* dst, const float* x) {
                                               pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRaThreads) rope_append_kernel(const RaParams p) {
-  __shared__ float2 cs[kRaMaxTokens][64];
-  __shared__ long long slot[kRaMaxTokens];  // pool slot, -1: k and v are not written, -2: the token is skipped
-  const int t0 = blockIdx.x * p.tokens_per_cta;
-  const int nt = min(p.tokens_per_cta, p.num_tokens - t0);
-  const int half = p.rotary_dim / 2;
+// How pairs lie in a head: on dims (2i, 2i + 1); on (i, i + R / 2) with both
+// halves whole vectors; or with halves that end inside a vector.
+enum { kRaInterleaved = 0, kRaHalves = 1, kRaOddHalves = 2 };
+
+// WARPS warps take a token (one: the CTA holds eight tokens).
+template <typename T, int MODE, int WARPS>
+__global__ void __launch_bounds__(kRaThreads, 4) rope_append_kernel(const RaParams p) {
+  constexpr int kLanes = 32 * WARPS, kRows = kLanes / kRaUnits;  // threads of a token, heads they have at a time
+  constexpr int kBatch = RaVec<T>::kBatch;
+  __shared__ float2 cs_all[kRaThreads / kLanes][64];  // of pair f at ra_at(f)
+  const int part = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const int t = blockIdx.x * (kRaThreads / kLanes) + part;
+  if (t >= p.num_tokens) return;  // whole warps; with several warps per token the grid is exact
+  const int H = p.n_heads, K = p.n_kv_heads, heads = H + 2 * K, half = p.rotary_dim / 2;
+  float2* cs = cs_all[part];
+  // element j of the eight threads of a head in eight neighbouring words
+  auto ra_at = [](int f) { return MODE == kRaInterleaved ? (f & 3) * 16 + (f >> 2) : (f & 7) * 8 + (f >> 3); };
+
+  // A thread keeps its unit u of a head's eight; va, vb: the unit's two vectors
+  // in a rotated head (in a V head u and u + 8).
+  const int u = lane % kRaUnits, pairs_r = p.rotary_dim / 16;
+  int va = u, vb = u + 8;
+  if (MODE == kRaHalves) {
+    va = u < pairs_r ? u : pairs_r + u;
+    vb = u < pairs_r ? u + pairs_r : u + 8;
+  }
+  auto source = [&](int h) {
+    return h < H       ? static_cast<const T*>(p.q) + t * p.q_stride + h * kHeadDim
+           : h < H + K ? static_cast<const T*>(p.k) + t * p.k_stride + (h - H) * kHeadDim
+                       : static_cast<const T*>(p.v) + t * p.v_stride + (h - H - K) * kHeadDim;
+  };
+  RaVec<T> a[kBatch], b[kBatch];
+  auto fetch = [&](int head) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = head + i * kRows;
+      if (h < heads) {
+        const T* src = source(h);
+        a[i].load(src + 8 * (h < H + K ? va : u));
+        b[i].load(src + 8 * (h < H + K ? vb : u + 8));
+      }
+    }
+  };
+
   pdl_wait();  // q, k, v come from the previous kernel
   pdl_launch_dependents();
-  if (threadIdx.x < nt) {
-    const int t = t0 + threadIdx.x;
-    const int seq = p.token_seq[t];
-    long long s = -1;
-    if (seq < 0) {
-      s = -2;
-    } else {
-      const int at = p.cache_index ? p.cache_index[t] : p.positions[t];
-      const int col = at >= 0 ? at / p.tokens_per_block : -1;
-      if (seq < p.num_seqs && col >= 0 && col < p.bt_stride) {
-        const int blk = p.block_table[(size_t)seq * p.bt_stride + col];
-        if (blk >= 0 && blk < p.num_blocks) s = (long long)blk * p.tokens_per_block + at % p.tokens_per_block;
-      }
-      if (s < 0) atomicOr(p.status, kStatusBadBlock);
-    }
-    slot[threadIdx.x] = s;
+  const int seq = p.token_seq[t], position = p.positions[t];
+  int head = lane / kRaUnits;
+  fetch(head);          // under way while the angles are computed
+  if (seq < 0) return;  // padding (all threads of the token)
+  long long slot = -1;  // in the pool; -1: k and v are not written
+  const int at = p.cache_index ? p.cache_index[t] : position;
+  const int col = at >= 0 ? at / p.tokens_per_block : -1;
+  if (seq < p.num_seqs && col >= 0 && col < p.bt_stride) {
+    const int blk = p.block_table[(size_t)seq * p.bt_stride + col];
+    if (blk >= 0 && blk < p.num_blocks)
+      slot = (long long)blk * p.tokens_per_block + (at - col * p.tokens_per_block);
   }
-  for (int i = threadIdx.x; i < nt * half; i += kRaThreads) {
-    const int t = i / half, f = i % half;
-    const double turns = (double)p.positions[t0 + t] * (p.inv_freq[f] * 0.15915494309189535);  // / 2 pi
+  if (slot < 0 && lane == 0) atomicOr(p.status, kStatusBadBlock);
+  for (int f = lane; f < half; f += kLanes) {
+    const double turns = (double)position * (p.inv_freq[f] * 0.15915494309189535);  // / 2 pi
     float sn, c;
     sincospif(2.f * (float)(turns - floor(turns)), &sn, &c);
-    cs[t][f] = make_float2(c * p.factor, sn * p.factor);
+    cs[ra_at(f)] = make_float2(c * p.factor, sn * p.factor);
   }
-  __syncthreads();
+  if (WARPS == 1)
+    __syncwarp();
+  else
+    __syncthreads();
 
-  const int H = p.n_heads, K = p.n_kv_heads;
-  const int per_token = (H + 2 * K) * kRaUnits;
-  const int vec_r = p.rotary_dim / 8, pairs_r = p.rotary_dim / 16;  // rotated vectors; half-split vector pairs
-  const bool aligned = p.rotary_dim % 16 == 0;
-  for (int i = threadIdx.x; i < nt * per_token; i += kRaThreads) {
-    const int tl = i / per_token, r = i % per_token;
-    const int head = r / kRaUnits, u = r % kRaUnits;
-    const long long s = slot[tl];
-    if (s == -2) continue;
-    const size_t t = (size_t)(t0 + tl);
-    const T* src;
-    __nv_bfloat16* dst;
-    if (head < H) {
-      src = static_cast<const T*>(p.q) + t * p.q_stride + head * kHeadDim;
-      dst = p.q_out + t * p.q_out_stride + head * kHeadDim;
-    } else {
-      if (s < 0) continue;
-      const bool is_v = head >= H + K;
-      const int kh = head - H - (is_v ? K : 0);
-      src = is_v ? static_cast<const T*>(p.v) + t * p.v_stride + kh * kHeadDim
-                 : static_cast<const T*>(p.k) + t * p.k_stride + kh * kHeadDim;
-      dst = p.pool + ((size_t)s * 2 * K + (is_v ? K : 0) + kh) * kHeadDim;
-    }
-    const bool rot = head < H + K;
-    // the unit's two vectors
-    int va = u, vb = u + 8;
-    if (rot && !p.interleaved && aligned) {
-      va = u < pairs_r ? u : vec_r + (u - pairs_r);
-      vb = u < pairs_r ? u + pairs_r : va + (8 - pairs_r);
-    }
-    float a[8], b[8];
-    ra_load8(src + 8 * va, a);
-    ra_load8(src + 8 * vb, b);
-    if (rot) {
-      const float2* cst = cs[tl];
-      if (p.interleaved) {
+  for (const int last = slot >= 0 ? heads : H; head < last;) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = head + i * kRows;
+      if (h >= last) break;
+      const bool rot = h < H + K;
+      __nv_bfloat16* dst = h < H ? p.q_out + t * p.q_out_stride + h * kHeadDim
+                                 // pool slot: K heads, then V heads
+                                 : p.pool + (slot * 2 * K + (h - H)) * kHeadDim;
+      float x[8], y[8];
+      a[i].get(x);
+      b[i].get(y);
+      if (rot && MODE == kRaInterleaved) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (8 * va + 2 * j < p.rotary_dim) {
-            const float2 w = cst[4 * va + j];
-            const float x = a[2 * j], y = a[2 * j + 1];
-            a[2 * j] = x * w.x - y * w.y;
-            a[2 * j + 1] = y * w.x + x * w.y;
+          if (4 * u + j < half) {
+            const float2 w = cs[16 * j + u];
+            const float c = x[2 * j], d = x[2 * j + 1];
+            x[2 * j] = c * w.x - d * w.y;
+            x[2 * j + 1] = d * w.x + c * w.y;
           }
-          if (8 * vb + 2 * j < p.rotary_dim) {
-            const float2 w = cst[4 * vb + j];
-            const float x = b[2 * j], y = b[2 * j + 1];
-            b[2 * j] = x * w.x - y * w.y;
-            b[2 * j + 1] = y * w.x + x * w.y;
+          if (4 * (u + 8) + j < half) {
+            const float2 w = cs[16 * j + u + 8];
+            const float c = y[2 * j], d = y[2 * j + 1];
+            y[2 * j] = c * w.x - d * w.y;
+            y[2 * j + 1] = d * w.x + c * w.y;
           }
         }
-      } else if (aligned) {
+      } else if (rot && MODE == kRaHalves) {
         if (u < pairs_r) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float2 w = cst[8 * va + j];
-            const float x = a[j], y = b[j];
-            a[j] = x * w.x - y * w.y;
-            b[j] = y * w.x + x * w.y;
+            const float2 w = cs[8 * j + u];
+            const float c = x[j], d = y[j];
+            x[j] = c * w.x - d * w.y;
+            y[j] = d * w.x + c * w.y;
           }
         }
-      } else {
+      } else if (rot) {
         // partners do not fall on vectors: fetch each one by itself
+        const T* src = source(h);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int da = 8 * va + j, db = 8 * vb + j;
-          if (da < p.rotary_dim) {
-            const int f = da < half ? da : da - half;
-            const float2 w = cst[f];
-            const float y = ra_load1(src + (da < half ? da + half : f));
-            a[j] = da < half ? a[j] * w.x - y * w.y : a[j] * w.x + y * w.y;
+          const int dx = 8 * u + j, dy = dx + 64;
+          if (dx < p.rotary_dim) {
+            const int f = dx < half ? dx : dx - half;
+            const float2 w = cs[ra_at(f)];
+            const float o = ra_load1(src + (dx < half ? dx + half : f));
+            x[j] = dx < half ? x[j] * w.x - o * w.y : x[j] * w.x + o * w.y;
           }
-          if (db < p.rotary_dim) {
-            const int f = db < half ? db : db - half;
-            const float2 w = cst[f];
-            const float y = ra_load1(src + (db < half ? db + half : f));
-            b[j] = db < half ? b[j] * w.x - y * w.y : b[j] * w.x + y * w.y;
+          if (dy < p.rotary_dim) {
+            const int f = dy < half ? dy : dy - half;
+            const float2 w = cs[ra_at(f)];
+            const float o = ra_load1(src + (dy < half ? dy + half : f));
+            y[j] = dy < half ? y[j] * w.x - o * w.y : y[j] * w.x + o * w.y;
           }
         }
       }
+      ra_store8(dst + 8 * (rot ? va : u), x);
+      ra_store8(dst + 8 * (rot ? vb : u + 8), y);
     }
-    ra_store8(dst + 8 * va, a);
-    ra_store8(dst + 8 * vb, b);
+    head += kBatch * kRows;
+    fetch(head);
   }
+}
+
+typedef void (*RaKernel)(const RaParams);
+template <typename T, int WARPS>
+RaKernel ra_kernel(const RaParams& p) {
+  if (p.interleaved) return rope_append_kernel<T, kRaInterleaved, WARPS>;
+  return p.rotary_dim % 16 == 0 ? rope_append_kernel<T, kRaHalves, WARPS> : rope_append_kernel<T, kRaOddHalves, WARPS>;
 }
 
 }  // namespace krt
@@ -269,9 +315,10 @@ extern "C" int krt_rope_append(const krt_rope_append_args* a, void* stream) {
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
   p.factor = a->factor == 0.f ? 1.f : a->factor;
-  p.tokens_per_cta = a->num_tokens >= kRaMaxTokens * 2 * device_sm_count() ? kRaMaxTokens : 1;
+  // A CTA per token while that leaves SMs free, then a warp per token.
+  const bool cta_each = a->num_tokens < 8 * device_sm_count();
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a->num_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta), 1, 1);
+  cfg.gridDim = dim3(cta_each ? (unsigned)a->num_tokens : ((unsigned)a->num_tokens + 7) / 8, 1, 1);
   cfg.blockDim = dim3(kRaThreads, 1, 1);
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];
@@ -279,8 +326,9 @@ extern "C" int krt_rope_append(const krt_rope_append_args* a, void* stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = dtype == KRT_DTYPE_FLOAT32 ? cudaLaunchKernelEx(&cfg, rope_append_kernel<float>, p)
-                                             : cudaLaunchKernelEx(&cfg, rope_append_kernel<__nv_bfloat16>, p);
+  RaKernel kern = dtype == KRT_DTYPE_FLOAT32 ? (cta_each ? ra_kernel<float, 8>(p) : ra_kernel<float, 1>(p))
+                                             : (cta_each ? ra_kernel<__nv_bfloat16, 8>(p) : ra_kernel<__nv_bfloat16, 1>(p));
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return cuda_error(e, name);
   return clear_error();
 }
