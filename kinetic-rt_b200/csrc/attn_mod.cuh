@@ -13,7 +13,6 @@ namespace krt {
 
 struct ScoreMod {
   float mul;         // scale * log2(e)
-  float2 mul2;       // the same twice
   float cap2;        // cap * log2(e), 0 = no cap
   float cap_in;      // 2 * log2(e) * scale / cap: ex2(s * cap_in) = e^(2 x / c)
   const float* slopes;  // [n_heads] or NULL
@@ -28,7 +27,6 @@ inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, 
   ScoreMod m;
   const float sc = scale > 0.f ? scale : 0.08838834764831845f;  // 1 / sqrt(128)
   m.mul = sc * kLog2e;
-  m.mul2 = make_float2(m.mul, m.mul);
   m.cap2 = softcap * kLog2e;
   m.cap_in = softcap > 0.f ? 2.f * kLog2e * sc / softcap : 0.f;
   m.slopes = slopes;

@@ -7,31 +7,45 @@
 //                             hi = min(len_s, max(p + 1, prefix_s))
 //   out = sum_j softmax(x)_j v_j,  lse = log sum_j exp(x_j);  nothing visible: 0 and -inf
 //
-// One CTA works on 256 rows = two tiles of 128 rows; a tile holds 128 / G
-// query tokens x the G query heads of one KV head (rows token-major), so a
-// K/V block that is fetched serves all of them.  Twelve warps:
-//   * warps 0-3 and 4-7: softmax of tile 0 and tile 1, one thread per row (TMEM
-//     lane), so maxima and sums need no exchange;
-//   * warps 8 and 11: TMA producers of K and of V.  Blocks of 64 tokens, 16 KB
-//     each, in two rings of five stages; a block is four 16-token pages, two
-//     boxes each;
-//   * warps 9 and 10: issue the UMMAs of tile 0 and tile 1: S = Q K^T (M = 128,
+// The unit of work (an item) is 256 rows of one KV head = two tiles of 128; a
+// tile holds 128 / G query tokens x the G query heads of the KV head (rows
+// token-major), so a K/V block that is fetched serves all of them.  A CTA per
+// SM takes items from a queue, the heaviest of a sequence first.  Its warps:
+//   * 0-3 and 4-7: softmax of tile 0 and tile 1, one thread per row (TMEM
+//     lane), so maxima and sums need no exchange; 168 registers each, the
+//     whole block of 64 scores stays in them;
+//   * 8: TMA producer of K, which also finds the next item while the present
+//     one is worked on; 11: producer of V.  Blocks of 64 tokens, 16 KB each, in
+//     two rings of four stages; a block is four 16-token pages, two boxes each;
+//   * 9 and 10: issue the UMMAs of tile 0 and tile 1: S = Q K^T (M = 128,
 //     N = 64, both operands in shared memory) and O += P V (P from TMEM, V as
 //     the MN-major operand).  Two warps, because the waits, descriptors and
 //     commits of a step take longer than its 12 MMAs (one warp for both tiles:
 //     2600 cycles a step, of which the tensor core worked half).
-// TMEM, per tile: two S buffers of 64 columns and O of 128 (all 512 columns).
-// P (bf16, 32 columns) overwrites its S.  Each tile has two blocks in flight:
-// while the softmax works on block g, the tensor core has P V of block g - 1
-// and Q K^T of block g + 1 of the same tile to do, and those of the other
-// tile.  With one buffer of 128 columns per tile the chain S -> weights -> P V
-// -> next S bounded the kernel (4150 cycles for 128 keys and both tiles, where
-// tensor core and special-function units need 2048 each).
+// Shared memory: Q 64 KB, rings 128 KB, output staging 32 KB.  TMEM, per tile:
+// two S buffers of 64 columns and O of 128 (all 512 columns).  P (bf16, 32
+// columns) overwrites its S.  Each tile has two blocks in flight: while the
+// softmax works on block g, the tensor core has P V of block g - 1 and Q K^T of
+// block g + 1 of the same tile to do, and those of the other tile.  With one
+// buffer of 128 columns per tile the chain S -> weights -> P V -> next S
+// bounded the kernel (4150 cycles for 128 keys and both tiles, where tensor
+// core and special-function units need 2048 each).
 //
-// What bounds it now: per 128 keys and pair of tiles the tensor core needs
-// about 2560 cycles (2048 of arithmetic; at N = 64 Q K^T reads 6 KB of shared
-// memory per 32 cycles of it), the special-function units 2048 for one ex2 a
-// score.  Steps that are spared:
+// Few rows behind a long cache make fewer items than there are SMs; their keys
+// are then split into pieces (of eight blocks at least), whose unnormalised
+// sums a second kernel joins.  Measured, 8 tokens of 8 KV heads behind 65536:
+// 726 us whole, 64 split; behind 8192: 100 and 25; behind 1024: 19 and 17.
+// (Pieces of four blocks: 14 there, but a 512-token prompt takes 20 for 17.)
+//
+// What bounds it: per 128 keys and pair of tiles the tensor core needs about
+// 2560 cycles (2048 of arithmetic; at N = 64 Q K^T reads 6 KB of shared memory
+// per 32 cycles of it), the special-function units 2048 for one ex2 a score.
+// A step takes about 3500 without and 4500 with a cap: the softmax warps' issue
+// slots (the cap's polynomial, maxima, packing) come on top of what the
+// special-function units leave of them.  Measured: six chunks of 517 tokens
+// behind 3700, 64 heads, 296 us = 957 TFLOP/s; 8 x 2048, 32 heads, causal,
+// capped, 357 us = 770 TFLOP/s; 64 tokens alone, 9.4 us in a graph.
+// Steps that are spared:
 //   * the reference that scores are taken against is the row's old maximum
 //     unless it grew by more than 2^8 (weights then stay below 256, and bf16
 //     and the fp32 sum lose nothing by it); only then O and the sum are
@@ -47,6 +61,7 @@
 // blocks that are not visible to all live rows, V values that are not finite
 // are set to 0 in shared memory before P V, and a CTA that found some adds
 // them in its epilogue to the rows that do see them.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -75,6 +90,11 @@ constexpr uint32_t kApmOutBytes = 16384;   // 64 columns of a tile's output
 constexpr float kApmLazy = 8.f;   // growth of a row's maximum (base 2) that is left unscaled
 constexpr float kApmBound = 50.f; // largest reference (base 2) that may lie above the row's maximum
 constexpr int kApmMaxPos = 1 << 30;
+constexpr int kApmMinPiece = 8;   // key blocks of a piece at least, where an item is split
+constexpr size_t kApmQueueAt = 256, kApmFlagsAt = 1024;  // in the workspace's header
+constexpr int kApmMaxPieces = (kWsHeaderBytes - kApmFlagsAt) / 8;
+constexpr size_t kApmPartBytes = (size_t)2 * kApmRows * kHeadDim * 4;  // a piece's O, both tiles
+constexpr size_t kApmStatBytes = (size_t)2 * kApmRows * 8;             // its references and sums
 
 struct ApmParams {
   __nv_bfloat16* out;
@@ -86,7 +106,11 @@ struct ApmParams {
   const int32_t* kv_start;
   const int32_t* prefix_lens;
   int* status;
-  uint32_t* queue;           // [next item, CTAs that are through], zero between launches
+  uint32_t* queue;           // [next piece, CTAs that are through], zero between launches
+  int items, splits;         // items, and pieces of each, at most
+  float4* part_o;            // [piece][tile][column / 4][row]
+  float2* part_ml;           // [piece][tile][row] reference and sum
+  int32_t* part_flags;       // [piece][tile] V values that are not finite were taken out
   int num_tokens, num_seqs, bt_stride, num_blocks, tokens_per_block;
   int n_kv_heads, group, tile_tokens;  // tile_tokens = 128 / group
   uint32_t group_inv;                  // row / group = row * group_inv >> 16 for rows below 128
@@ -94,8 +118,8 @@ struct ApmParams {
   ScoreMod mod;
 };
 
-// One piece of work: a pair of tiles of one sequence and KV head.  Filled in by
-// the scheduling warp one item ahead of the others.
+// A piece of work: a pair of tiles of one sequence and KV head, and their keys
+// or a part of those.  Filled in by the scheduling warp one ahead of the others.
 struct ApmItem {
   int seq;                // -1: there is no more work
   int kvh;
@@ -105,6 +129,7 @@ struct ApmItem {
   int first[2], end[2];   // key blocks of each tile, [first, end); both 0 without a live row
   int lo_all, hi_all;     // keys that some live row sees
   int lo_max, hi_min;     // keys that all live rows see
+  int part;               // where the piece leaves its part of the result, -1: it is the whole item
 };
 
 struct ApmSmemTail {
@@ -153,7 +178,8 @@ __device__ __forceinline__ int apm_lowest(const ApmParams& p, int pos) {
   return p.mod.window > 0 ? max(0, pos - p.mod.window + 1) : 0;
 }
 
-// Item number `index` (seq -1: there are fewer): sequences in order, the last
+// Item number `index` (seq -1: there are fewer, or q_start decreases somewhere
+// and they are more than num_tokens rows can give): sequences in order, the last
 // (heaviest) tokens of each first, KV heads innermost.  By a whole warp, 128
 // sequences at a time, so that their loads overlap.
 __device__ __forceinline__ ApmItem apm_find(const ApmParams& p, int index, int lane) {
@@ -161,7 +187,7 @@ __device__ __forceinline__ ApmItem apm_find(const ApmParams& p, int index, int l
   const int kvh = index % p.n_kv_heads, target = index / p.n_kv_heads;
   int seq = -1, t_first = 0, q_len = 0, pos0 = 0, tok0 = 0, base = 0;
 #pragma unroll 1
-  for (int s0 = 0; s0 < p.num_seqs && seq < 0; s0 += 128) {
+  for (int s0 = 0; s0 < p.num_seqs && seq < 0 && index < p.items; s0 += 128) {
     int a[4], e[4], p0[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -245,7 +271,50 @@ __device__ __forceinline__ ApmItem apm_find(const ApmParams& p, int index, int l
     it.hi_all = max(it.hi_all, hi_max);
   }
   if (it.hi_all == 0) it.lo_all = 0;
+  it.part = -1;
   return it;
+}
+
+// Key blocks per piece of the item, and how many pieces that makes.
+__device__ __forceinline__ int apm_pieces(const ApmParams& p, const ApmItem& it, int* len) {
+  const int blocks = (it.hi_all + kApmBlock - 1) / kApmBlock - it.lo_all / kApmBlock;
+  *len = max(kApmMinPiece, (blocks + p.splits - 1) / p.splits);
+  return max(1, (blocks + *len - 1) / *len);
+}
+
+// Cuts the item down to its piece z.
+__device__ __forceinline__ void apm_cut(ApmItem& it, int z, int len, int part) {
+  const int b0 = it.lo_all / kApmBlock + z * len, b1 = b0 + len;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    it.first[i] = max(it.first[i], b0);
+    it.end[i] = min(it.end[i], b1);
+    if (it.first[i] >= it.end[i]) it.first[i] = it.end[i] = 0;
+  }
+  it.lo_all = max(it.lo_all, b0 * kApmBlock);
+  it.hi_all = (int)min((long long)it.hi_all, (long long)b1 * kApmBlock);
+  it.part = part;
+}
+
+// Adds the V values that were taken out (dims d0 .. d1 - 1) to a row that sees them.
+__device__ __forceinline__ void apm_add_back(const ApmParams& p, const ApmItem* at, int lo, int hi, __nv_bfloat16* out,
+                                             int d0, int d1) {
+#pragma unroll 1
+  for (int j = lo; j < hi; ++j) {
+    const int j0 = j / kApmBlock * kApmBlock;
+    if (j0 >= at->lo_max && j0 + kApmBlock <= at->hi_min) {  // a block that was not cleaned
+      j = j0 + kApmBlock - 1;
+      continue;
+    }
+    const long long sl = apm_slot(p, p.block_table + (size_t)at->seq * p.bt_stride, j);
+    if (sl < 0) continue;
+    const __nv_bfloat16* v = p.pool + ((size_t)sl * 2 * p.n_kv_heads + p.n_kv_heads + at->kvh) * kHeadDim;
+#pragma unroll 1
+    for (int i = d0; i < d1; ++i) {
+      const float f = __bfloat162float(v[i]);
+      if (!isfinite(f)) out[i] = __float2bfloat16(__bfloat162float(out[i]) + f);
+    }
+  }
 }
 
 template <bool CAP, bool BIAS>
@@ -330,11 +399,24 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       ApmItem it;
       if (kv == 0) {
         uint32_t index = blockIdx.x;
-        if (k > 0) {
-          if (lane == 0) index = gridDim.x + atomicAdd(p.queue, 1u);
-          index = __shfl_sync(0xffffffffu, index, 0);
+        bool queued = k > 0;
+#pragma unroll 1
+        while (true) {
+          if (queued) {
+            if (lane == 0) index = gridDim.x + atomicAdd(p.queue, 1u);
+            index = __shfl_sync(0xffffffffu, index, 0);
+          }
+          const int z = (int)(index % p.splits);
+          it = apm_find(p, (int)(index / p.splits), lane);
+          if (p.splits == 1 || it.seq < 0) break;
+          int len;
+          const int pieces = apm_pieces(p, it, &len);
+          if (z < pieces) {
+            if (pieces > 1) apm_cut(it, z, len, (int)index);
+            break;
+          }
+          queued = true;  // the item has fewer pieces
         }
-        it = apm_find(p, (int)index, lane);
         if (k > 1 && !mbar_wait_all(&tl->item_empty[k & 1], (uint32_t)((k >> 1) - 1) & 1u, abort_flag)) {
           if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
           break;
@@ -744,69 +826,73 @@ __global__ void __launch_bounds__(kApmThreads, 1)
         ++last;
         partial_pv += n - 1;
       }
-      const int t = at->t_first + tok, head = at->kvh * G + r - row_tok * G;
-      const float inv = !live || l == 0.f ? 0.f : 1.f / l;
-      // Through shared memory, 64 columns at a time (16-byte pieces, 128-byte
-      // swizzle), then whole rows: a row written by its thread alone would take
-      // a memory transaction for every 16 bytes.
-      uint8_t* stage = out_smem + wg * kApmOutBytes;
-      const int rows = min(tt, at->q_len - at->tok0 - wg * tt) * G;  // rows of the tile that exist
-      __nv_bfloat16* tile_out = p.out + (size_t)(at->t_first + at->tok0 + wg * tt) * p.out_stride +
-                                (size_t)at->kvh * G * kHeadDim + (lane & 7) * 8;
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        float o[64];
+      if (at->part >= 0) {
+        // a piece: the row's unnormalised sums for the kernel that joins them
+        const size_t tile = (size_t)at->part * 2 + wg;
+        if (valid) p.part_ml[tile * kApmRows + r] = live ? make_float2(m_ref, l) : make_float2(-INFINITY, 0.f);
+        if (r == 0) p.part_flags[tile] = *reinterpret_cast<volatile int*>(&tl->poison[k & 1]) == k + 1;
         if (n > 0) {
-          tmem_ld32_nowait(o_addr + 64 * c, o);
-          tmem_ld32_nowait(o_addr + 64 * c + 32, o + 32);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) o[i] = 0.f;
-        }
-        tmem_wait_ld64(o);
-        __syncwarp();  // the warp's rows of the first 64 columns are read
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = live ? pack_bf16x2(o[8 * i + 2 * e] * inv, o[8 * i + 2 * e + 1] * inv) : 0u;
-          *reinterpret_cast<uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int rr = (warp & 3) * 32 + 4 * i + (lane >> 3), tk = (int)(rr * p.group_inv >> 16);
-          if (rr < rows)
-            *reinterpret_cast<uint4*>(tile_out + (size_t)tk * p.out_stride + (rr - tk * G) * kHeadDim + 64 * c) =
-                *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-        }
-      }
-      // (O is read: the next item's first P, which its P V waits for, comes later)
-      __syncwarp();  // (the row may have been written by other lanes)
-      if (live && *reinterpret_cast<volatile int*>(&tl->poison[k & 1]) == k + 1) {
-        // V values that were taken out, to the rows that see them
-        __nv_bfloat16* out = p.out + (size_t)t * p.out_stride + (size_t)head * kHeadDim;
+          float4* dst = p.part_o + tile * (kHeadDim / 4) * kApmRows + r;
 #pragma unroll 1
-        for (int j = lo; j < hi; ++j) {
-          const int j0 = j / kApmBlock * kApmBlock;
-          if (j0 >= at->lo_max && j0 + kApmBlock <= at->hi_min) {  // a block that was not cleaned
-            j = j0 + kApmBlock - 1;
-            continue;
-          }
-          const long long sl = apm_slot(p, p.block_table + (size_t)at->seq * p.bt_stride, j);
-          if (sl < 0) continue;
-          const __nv_bfloat16* v = p.pool + ((size_t)sl * 2 * p.n_kv_heads + p.n_kv_heads + at->kvh) * kHeadDim;
-#pragma unroll 1
-          for (int i = 0; i < kHeadDim; ++i) {
-            const float f = __bfloat162float(v[i]);
-            if (!isfinite(f)) out[i] = __float2bfloat16(__bfloat162float(out[i]) + f);
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            tmem_ld32_nowait(o_addr + 32 * c, o);
+            tmem_wait_ld32(o);
+            if (valid) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                dst[(8 * c + i) * kApmRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
           }
         }
+      } else {
+        const int t = at->t_first + tok, head = at->kvh * G + r - row_tok * G;
+        const float inv = !live || l == 0.f ? 0.f : 1.f / l;
+        // Through shared memory, 64 columns at a time (16-byte pieces, 128-byte
+        // swizzle), then whole rows: a row written by its thread alone would take
+        // a memory transaction for every 16 bytes.
+        uint8_t* stage = out_smem + wg * kApmOutBytes;
+        const int rows = min(tt, at->q_len - at->tok0 - wg * tt) * G;  // rows of the tile that exist
+        __nv_bfloat16* tile_out = p.out + (size_t)(at->t_first + at->tok0 + wg * tt) * p.out_stride +
+                                  (size_t)at->kvh * G * kHeadDim + (lane & 7) * 8;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          float o[64];
+          if (n > 0) {
+            tmem_ld32_nowait(o_addr + 64 * c, o);
+            tmem_ld32_nowait(o_addr + 64 * c + 32, o + 32);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] = 0.f;
+          }
+          tmem_wait_ld64(o);
+          __syncwarp();  // the warp's rows of the first 64 columns are read
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = live ? pack_bf16x2(o[8 * i + 2 * e] * inv, o[8 * i + 2 * e + 1] * inv) : 0u;
+            *reinterpret_cast<uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = (warp & 3) * 32 + 4 * i + (lane >> 3), tk = (int)(rr * p.group_inv >> 16);
+            if (rr < rows)
+              *reinterpret_cast<uint4*>(tile_out + (size_t)tk * p.out_stride + (rr - tk * G) * kHeadDim + 64 * c) =
+                  *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+          }
+        }
+        // (O is read: the next item's first P, which its P V waits for, comes later)
+        __syncwarp();  // (the row may have been written by other lanes)
+        if (live && *reinterpret_cast<volatile int*>(&tl->poison[k & 1]) == k + 1) {
+          apm_add_back(p, at, lo, hi, p.out + (size_t)t * p.out_stride + (size_t)head * kHeadDim, 0, kHeadDim);
+        }
+        if (valid && p.lse)
+          p.lse[(size_t)t * p.lse_stride + head] =
+              !live || l == 0.f ? -INFINITY : (m_ref == -INFINITY ? l : (m_ref + log2f(l)) * kLn2);
       }
-      if (valid && p.lse)
-        p.lse[(size_t)t * p.lse_stride + head] =
-            !live || l == 0.f ? -INFINITY : (m_ref == -INFINITY ? l : (m_ref + log2f(l)) * kLn2);
       done += n;
       blocks += (at->hi_all + kApmBlock - 1) / kApmBlock - g0;
       release_item(k);
@@ -829,6 +915,66 @@ __global__ void __launch_bounds__(kApmThreads, 1)
   }
 }
 
+// Joins the pieces of the items that were split.  A CTA takes 32 rows of a tile,
+// a thread 16 dims of one row, so that a warp reads whole lines of the parts.
+__global__ void __launch_bounds__(256) paged_attention_prefill_mod_join_kernel(const __grid_constant__ ApmParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int item = blockIdx.x >> 3, i = (blockIdx.x >> 2) & 1, r = (blockIdx.x & 3) * 32 + lane;
+  pdl_wait();
+  pdl_launch_dependents();
+  const ApmItem it = apm_find(p, item, lane);
+  if (it.seq < 0) return;
+  int len;
+  const int pieces = apm_pieces(p, it, &len);
+  const int tok_in = (int)(r * p.group_inv >> 16), tok = it.tok0 + i * p.tile_tokens + tok_in;
+  if (pieces == 1 || r >= p.tile_tokens * p.group || tok >= it.q_len) return;
+  const size_t tile0 = (size_t)item * p.splits * 2 + i;  // of piece 0; the next piece's is 2 on
+  const float2* ml = p.part_ml + tile0 * kApmRows + r;
+  const float4* po = p.part_o + (tile0 * (kHeadDim / 4) + 4 * warp) * kApmRows + r;
+  float M = -INFINITY, L = 0.f, acc[16];
+  int poison = 0;
+#pragma unroll 4
+  for (int z = 0; z < pieces; ++z) {
+    M = fmaxf(M, __ldcg(&ml[(size_t)z * 2 * kApmRows]).x);
+    poison |= __ldcg(&p.part_flags[tile0 + 2 * z]);
+  }
+  const float mu = M == -INFINITY ? 0.f : M;  // nothing seen, or only NaN
+#pragma unroll
+  for (int d = 0; d < 16; ++d) acc[d] = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < pieces; ++z) {
+    const float2 w = __ldcg(&ml[(size_t)z * 2 * kApmRows]);
+    float4 o[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = __ldcg(&po[((size_t)z * 2 * (kHeadDim / 4) + c) * kApmRows]);
+    if (w.x == -INFINITY && w.y == 0.f) continue;  // the row sees nothing of the piece; O may not be set
+    const float f = ex2(w.x - mu);
+    L += f * w.y;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      acc[4 * c] += f * o[c].x;
+      acc[4 * c + 1] += f * o[c].y;
+      acc[4 * c + 2] += f * o[c].z;
+      acc[4 * c + 3] += f * o[c].w;
+    }
+  }
+  const int t = it.t_first + tok, head = it.kvh * p.group + r - tok_in * p.group, pos = it.pos0 + tok;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  uint32_t w[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) w[d] = pack_bf16x2(acc[2 * d] * inv, acc[2 * d + 1] * inv);
+  __nv_bfloat16* out = p.out + (size_t)t * p.out_stride + (size_t)head * kHeadDim;
+  uint4* dst = reinterpret_cast<uint4*>(out + 16 * warp);
+  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  if (poison) {
+    const int lo = max(apm_lowest(p, pos), p.kv_start ? p.kv_start[t] : 0);
+    apm_add_back(p, &it, lo, min(it.pos0 + it.q_len, max(pos + 1, it.prefix)), out, 16 * warp, 16 * warp + 16);
+  }
+  if (p.lse && warp == 0)
+    p.lse[(size_t)t * p.lse_stride + head] = L == 0.f ? -INFINITY : (M == -INFINITY ? L : (M + log2f(L)) * kLn2);
+}
+
 typedef void (*ApmKernel)(const CUtensorMap, const CUtensorMap, const ApmParams);
 ApmKernel apm_kernel(bool cap, bool bias) {
   if (cap)
@@ -840,13 +986,35 @@ ApmKernel apm_kernel(bool cap, bool bias) {
 
 using namespace krt;
 
+namespace {
+
+// Items (pairs of tiles of a KV head) of a call at most, however its tokens
+// fall on the sequences.
+long long apm_items(int num_tokens, int num_seqs, int n_heads, int n_kv_heads) {
+  const int tile_tokens = kApmRows / (n_heads / n_kv_heads);
+  return (num_tokens / (2 * tile_tokens) + (long long)num_seqs) * n_kv_heads;
+}
+
+int apm_max_pieces() { return std::min(device_sm_count(), kApmMaxPieces); }
+
+// Pieces that an item of so many key blocks is worth at most.
+long long apm_worth(long long blocks) { return (blocks + kApmMinPiece - 1) / kApmMinPiece; }
+
+long long apm_blocks(long long keys) { return (keys + kApmBlock - 1) / kApmBlock; }
+
+}  // namespace
+
 // ------------------------------------------------------------------ C ABI
 extern "C" size_t krt_paged_attention_prefill_mod_workspace_size(int32_t num_tokens, int32_t num_seqs, int32_t n_heads,
                                                                  int32_t n_kv_heads, int32_t max_kv_len) {
   if (num_tokens <= 0 || num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 ||
       max_kv_len <= 0)
     return 0;
-  return kWsHeaderBytes;  // status word, and the queue behind it
+  // status word, queue and flags; parts of items that are split
+  const long long items = apm_items(num_tokens, num_seqs, n_heads, n_kv_heads);
+  const long long worth = apm_worth(apm_blocks(max_kv_len));
+  const size_t pieces = worth > 1 ? (size_t)std::min<long long>(apm_max_pieces(), items * worth) : 0;
+  return kWsHeaderBytes + pieces * (kApmPartBytes + kApmStatBytes);
 }
 
 extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention_mod_args* a, void* stream) {
@@ -893,7 +1061,9 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   p.kv_start = a->kv_start;
   p.prefix_lens = a->prefix_lens;
   p.status = static_cast<int*>(a->workspace);
-  p.queue = reinterpret_cast<uint32_t*>(static_cast<char*>(a->workspace) + 256);
+  char* ws = static_cast<char*>(a->workspace);
+  p.queue = reinterpret_cast<uint32_t*>(ws + kApmQueueAt);
+  p.part_flags = reinterpret_cast<int32_t*>(ws + kApmFlagsAt);
   p.num_tokens = a->num_tokens;
   p.num_seqs = a->num_seqs;
   p.bt_stride = a->block_table_stride;
@@ -906,9 +1076,15 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   p.out_stride = a->out_stride;
   p.lse_stride = a->lse_stride;
   p.mod = make_score_mod(a->scale, a->softcap, a->alibi_slopes, a->window);
-  // at most this many pairs of tiles over all sequences, however the tokens fall on them
-  const long long tiles = a->num_tokens / (2 * p.tile_tokens) + (long long)a->num_seqs;
-  if (tiles * a->n_kv_heads > INT_MAX) return set_error(KRT_ERR_UNSUPPORTED, "%s: too many tokens or heads", name);
+  const long long items = apm_items(a->num_tokens, a->num_seqs, a->n_heads, a->n_kv_heads), sms = device_sm_count();
+  if (items > INT_MAX) return set_error(KRT_ERR_UNSUPPORTED, "%s: too many tokens or heads", name);
+  // Few rows before a long cache: their keys are split so that all SMs work.
+  long long blocks = apm_blocks(a->max_kv_len);
+  if (a->window > 0) blocks = std::min(blocks, apm_blocks((long long)a->window + 2 * p.tile_tokens) + 1);
+  p.items = (int)items;
+  p.splits = (int)std::max(1ll, std::min(apm_max_pieces() / items, apm_worth(blocks)));
+  p.part_ml = reinterpret_cast<float2*>(ws + kWsHeaderBytes);
+  p.part_o = reinterpret_cast<float4*>(ws + kWsHeaderBytes + (size_t)items * p.splits * kApmStatBytes);
   CUtensorMap tmap_q, tmap_kv;
   int rc = make_tmap_bf16_5d_strided(&tmap_q, a->q, {64, (uint64_t)a->n_heads, (uint64_t)a->num_tokens, 2},
                                      {256, (uint64_t)a->q_stride * 2, 128},
@@ -921,8 +1097,7 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_error(e, name);
   cudaLaunchConfig_t cfg = {};
-  const long long items = tiles * a->n_kv_heads, sms = device_sm_count();
-  cfg.gridDim = dim3((unsigned)(items < sms ? items : sms), 1, 1);
+  cfg.gridDim = dim3((unsigned)std::min(items * p.splits, sms), 1, 1);
   cfg.blockDim = dim3(kApmThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
@@ -932,6 +1107,12 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kern, tmap_q, tmap_kv, p);
+  if (e == cudaSuccess && p.splits > 1) {
+    cfg.gridDim = dim3((unsigned)items * 8, 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, paged_attention_prefill_mod_join_kernel, p);
+  }
   if (e != cudaSuccess) return cuda_error(e, name);
   return clear_error();
 }

@@ -326,8 +326,9 @@ extern "C" int krt_rope_append(const krt_rope_append_args* a, void* stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  RaKernel kern = dtype == KRT_DTYPE_FLOAT32 ? (cta_each ? ra_kernel<float, 8>(p) : ra_kernel<float, 1>(p))
-                                             : (cta_each ? ra_kernel<__nv_bfloat16, 8>(p) : ra_kernel<__nv_bfloat16, 1>(p));
+  RaKernel kern = dtype == KRT_DTYPE_FLOAT32
+                      ? (cta_each ? ra_kernel<float, 8>(p) : ra_kernel<float, 1>(p))
+                      : (cta_each ? ra_kernel<__nv_bfloat16, 8>(p) : ra_kernel<__nv_bfloat16, 1>(p));
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return cuda_error(e, name);
   return clear_error();

@@ -581,7 +581,8 @@ def prefill_attention_mod_args(q, kv_pool, block_table, q_start, q_pos0, out, n_
     a.scale, a.softcap = float(scale), float(softcap)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()
-    return _keep(a, device, q, kv_pool, block_table, q_start, q_pos0, out, lse, alibi_slopes, kv_start, prefix_lens, workspace)
+    return _keep(a, device, q, kv_pool, block_table, q_start, q_pos0, out, lse, alibi_slopes, kv_start, prefix_lens,
+                 workspace)
 
 
 def paged_attention_prefill_mod(args, stream=None):
@@ -631,7 +632,8 @@ def rope_append_args(q, k, v, inv_freq, positions, token_seq, block_table, kv_po
     a.num_blocks, a.tokens_per_block, a.factor = int(num_blocks), int(tokens_per_block), float(factor)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()
-    return _keep(a, device, q, k, v, inv_freq, positions, cache_index, token_seq, block_table, kv_pool, q_out, workspace)
+    return _keep(a, device, q, k, v, inv_freq, positions, cache_index, token_seq, block_table, kv_pool, q_out,
+                 workspace)
 
 
 def rope_append(args, stream=None):

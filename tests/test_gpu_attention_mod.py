@@ -409,3 +409,64 @@ def test_decode_sizes_share_a_workspace(torch_cuda, seqs, ctx, H, K):
         seen = ~np.isneginf(lse)
         assert (np.isneginf(got_lse) == ~seen).all()
         assert (np.abs(got_lse[seen] - lse[seen]) <= np.broadcast_to(tol_lse, lse.shape)[seen]).all()
+
+
+# Few rows behind a long cache: the keys of an item are split over CTAs and joined.
+@pytest.mark.parametrize("softcap,bias,window", [(0.0, False, 0), (30.0, False, 0), (0.0, True, 0), (50.0, True, 1500)])
+@pytest.mark.parametrize("H,K", [(8, 2), (5, 1), (16, 1)])
+def test_prefill_few_rows_long_cache(torch_cuda, H, K, softcap, bias, window):
+    """Sequences of many pieces, of two, of one, and of none."""
+    c = Case(torch_cuda, [9000, 1, 1100, 0, 513], q_lens=[7, 30, 1, 0, 70], n_heads=H, n_kv_heads=K, seed=31 + H,
+             q_pad=8, rows_pad=5)
+    c.check(softcap=softcap, slopes=slopes_of(H) if bias else None, window=window)
+
+
+def test_prefill_few_rows_prefix_and_starts(torch_cuda):
+    """Rows whose keys lie in some of the pieces only, rows that see nothing, and a prefix beyond the rows' positions."""
+    c = Case(torch_cuda, [5000, 2500], q_lens=[40, 3], seed=32)
+    start = [0, 4990, 1 << 30, 3000, 5001] * 8 + [0, 2400, 2 ** 31 - 1]
+    c.check(kv_start=start, prefix=[0, 2503])
+    c.check(kv_start=start, softcap=20.0)
+    c.check(kv_start=[1 << 30] * 43)
+
+
+def test_prefill_few_rows_not_finite(torch_cuda):
+    """V values that are not finite, in blocks that only some rows see, reach the rows that see them across pieces."""
+
+    def edit(pool, c):
+        for j, d, v in ((700, 3, np.nan), (2900, 4, np.inf), (4003, 5, -np.inf), (4010, 6, np.nan)):
+            b, o = c.slot(0, j)
+            pool[b, o, 1, 0, d] = v
+
+    c = Case(torch_cuda, [4000], q_lens=[12], seed=33, edit_pool=edit)
+    start = [0, 701, 2901, 4004] * 3
+    c.launch(c.args(kv_start=start))
+    got, lse = c.result()
+    want = np.zeros(got.shape, bool)
+    for r in range(12):
+        for j, d in ((700, 3), (2900, 4), (4003, 5), (4010, 6)):
+            want[r, :4, d] = start[r] <= j <= 4000 + r
+    assert (~np.isfinite(got) == want).all()
+    assert (np.isfinite(lse).all(axis=1) == [start[r] <= 4000 + r for r in range(12)]).all()  # row 3 sees nothing
+    clean = np.where(np.isfinite(c.pool), c.pool, 0)
+    ref, _, tol, _ = orc.paged_attention_mod(c.q, clean, c.table, c.rows(start), c.H, c.K, 16)
+    assert (np.abs(np.where(want, 0, got) - np.where(want, 0, ref)) <= tol).all()
+
+
+def test_prefill_sizes_share_a_workspace(torch_cuda):
+    """One workspace, made for the largest call, serves split and whole items in turn."""
+    from python.kinetic_rt import _lib
+    ws = torch_cuda.zeros(_lib.prefill_attention_mod_workspace_bytes(4096, 16, 8, 2, 8192), dtype=torch_cuda.uint8,
+                          device="cuda")
+    for ctx, q_lens in (([4000, 0], [9, 2]), ([0] * 9, [600] * 9), ([8000], [3]), ([4000, 0], [9, 2])):
+        case = Case(torch_cuda, ctx, q_lens=q_lens, seed=34)
+        a = case.args()
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        case.launch(a)
+        rc, bits = _lib.read_status(ws)
+        assert rc == 0 and bits == 0
+        rows = [r if t % 61 == 0 else None for t, r in enumerate(case.rows())]
+        ref, lse, tol, tol_lse = orc.paged_attention_mod(case.q, case.pool, case.table, rows, 8, 2, 16)
+        got, got_lse = case.result()
+        assert (np.abs(got - ref) <= tol)[::61].all()
+        assert (np.abs(got_lse - lse) <= tol_lse)[::61].all()
