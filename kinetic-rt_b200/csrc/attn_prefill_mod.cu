@@ -47,7 +47,7 @@
 // capped, 357 us = 770 TFLOP/s; 64 tokens alone, 9.4 us in a graph.
 // Steps that are spared:
 //   * the reference that scores are taken against is the row's old maximum
-//     unless it grew by more than 2^8 (weights then stay below 256, and bf16
+//     unless it grew by more than 2^16 (weights then stay below that, and bf16
 //     and the fp32 sum lose nothing by it); only then O and the sum are
 //     rescaled, after the tile's last P V;
 //   * the cap is a polynomial of the score while scores are well below it, and
@@ -87,7 +87,7 @@ constexpr uint32_t kApmHalf = 16384;
 constexpr uint32_t kApmKvBytes = 16384;    // K or V block: 64 tokens x 128 dims, two [64 x 128 B] halves
 constexpr uint32_t kApmKvHalf = 8192;
 constexpr uint32_t kApmOutBytes = 16384;   // 64 columns of a tile's output
-constexpr float kApmLazy = 8.f;   // growth of a row's maximum (base 2) that is left unscaled
+constexpr float kApmLazy = 16.f;   // growth of a row's maximum (base 2) that is left unscaled
 constexpr float kApmBound = 50.f; // largest reference (base 2) that may lie above the row's maximum
 constexpr int kApmMaxPos = 1 << 30;
 constexpr int kApmMinPiece = 8;   // key blocks of a piece at least, where an item is split
