@@ -472,16 +472,16 @@ def _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_h
 
 
 def _launch(who, fn, args, stream):
-    """Launches go to the current device's current stream: the tensors live
-    there.  A decode loop pays for every call, so the struct's byref and its
-    device index are kept with it and the stream is read as a raw handle."""
+    """Launches go to the current device, where the tensors must live, on its
+    current stream or the given one (a handle, as for the other calls).  A
+    decode loop pays for every call, so the struct's byref and its device index
+    are kept with it and the stream is read as a raw handle."""
     import torch
-    if stream is None:
-        device = torch._C._cuda_getDevice()
-        if device != args._index:
-            raise ValueError(f"{who}: the tensors are on cuda:{args._index}, the current device is cuda:{device} "
-                             "(torch.cuda.set_device)")
-        stream = torch._C._cuda_getCurrentRawStream(device)
+    device = torch._C._cuda_getDevice()
+    if device != args._index:
+        raise ValueError(f"{who}: the tensors are on cuda:{args._index}, the current device is cuda:{device} "
+                         "(torch.cuda.set_device)")
+    stream = torch._C._cuda_getCurrentRawStream(device) if stream is None else int(stream)
     rc = fn(args._ref, stream)
     if rc != KRT_OK:
         check(rc)

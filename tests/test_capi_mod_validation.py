@@ -150,3 +150,16 @@ def test_python_arguments_must_be_cuda_tensors():
     with pytest.raises(ValueError, match="CUDA device"):
         _lib.rope_append_args(bf(2, 512), bf(2, 128), bf(2, 128), torch.zeros(64, dtype=torch.float64), i32(2), i32(2),
                               i32(1, 2), bf(4, 16, 2, 1, 128), bf(2, 512), 4, 1, 4, 16, ws)
+
+
+@pytest.mark.parametrize("stream", [None, 0, 77])
+@pytest.mark.parametrize("call", [_lib.paged_attention_decode_mod, _lib.paged_attention_prefill_mod, _lib.rope_append])
+def test_another_current_device_is_refused(monkeypatch, call, stream):
+    """A launch would run on the current device: with tensors of another one it does not start."""
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1, raising=False)
+    args = _lib.RopeAppendArgs()
+    args._index = 0
+    args._ref = None
+    with pytest.raises(ValueError, match="current device is cuda:1"):
+        call(args, stream)

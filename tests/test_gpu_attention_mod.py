@@ -470,3 +470,12 @@ def test_prefill_sizes_share_a_workspace(torch_cuda):
         got, got_lse = case.result()
         assert (np.abs(got - ref) <= tol)[::61].all()
         assert (np.abs(got_lse - lse) <= tol_lse)[::61].all()
+
+
+def test_prefill_many_sequences(torch_cuda):
+    """More sequences than the search for the work takes in one pass, empty ones among them."""
+    rng = np.random.Generator(np.random.PCG64(40))
+    q_lens = [int(n) for n in rng.choice([0, 1, 1, 2, 40], 300)]
+    c = Case(torch_cuda, [int(n) for n in rng.integers(0, 60, 300)], q_lens=q_lens, n_heads=4, n_kv_heads=2, seed=41,
+             rows_pad=3)
+    c.check(softcap=30.0)
