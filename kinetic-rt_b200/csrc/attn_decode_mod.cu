@@ -45,7 +45,7 @@ constexpr int kAdmChunk = 16;               // tokens per TMA box
 constexpr uint32_t kAdmStageBytes = 8192;   // K and V of 16 tokens, one KV head
 constexpr int kAdmMaxGroup = 16;            // query heads per KV head
 constexpr int kAdmRowFloats = 4 + kHeadDim; // max, sum, (two unused), 128 outputs
-constexpr int kAdmMaxCps = 512;             // 16-token chunks per CTA at most
+constexpr int kAdmMaxCps = 1024;            // 16-token chunks per CTA at most
 
 struct AdmParams {
   const __nv_bfloat16* q;
@@ -443,25 +443,27 @@ int adm_max_chunks(int max_seq_len, int window) {
 }
 
 // CTAs per (sequence, KV head): as many as fill the SMs once, but at most
-// sqrt(chunks) / 2 (the merge grows with their number as the scan shrinks),
-// and at least so many that none scans more than kAdmMaxCps chunks.  More,
-// smaller pieces lose: every CTA starts its pipeline, merges its warps and
-// leaves an fp32 partial.  Measured (us), pairs x chunks, this rule against
+// sqrt(chunks) / 2 (the merge grows with their number as the scan shrinks).
+// More, smaller pieces lose: every CTA starts its pipeline, merges its warps
+// and leaves an fp32 partial.  Measured (us), pairs x chunks, this rule against
 // two CTAs per SM and more: 256 x 65 25.6 : 31.0, 160 x 63 17.5 : 25.6,
 // 128 x 128 26.0 : 31.7, 8 x 512 14.7 : 17.1 (37 splits 26.8),
-// 8 x 264 11.1 : 17.5, 24 x 4096 of ragged lengths 132 : 133 to 139.
+// 8 x 264 11.1 : 17.5.  Long scans that leave a tenth of the SMs idle are cut
+// at 512 chunks, which evens out ragged lengths: 40 x 4096 177 : 190,
+// 90 x 2048 187 : 205; where the SMs are full they are not: 24 x 4096
+// 129 : 133.
 int adm_splits(long long pairs, int max_chunks) {
-  const int deepest = (max_chunks + kAdmMaxCps - 1) / kAdmMaxCps;
-  const long long fill = device_sm_count() / pairs;
-  const int most = (int)(std::sqrt((double)max_chunks) / 2);
-  return std::max(deepest, (int)std::min<long long>(fill, most));
+  const long long sms = device_sm_count(), most = (long long)(std::sqrt((double)max_chunks) / 2);
+  const long long s = std::max(1ll, std::min(sms / pairs, most));
+  const int deepest = 10 * s * pairs >= 9 * sms && s * pairs <= sms ? kAdmMaxCps : kAdmMaxCps / 2;
+  return (int)std::max<long long>(s, (max_chunks + deepest - 1) / deepest);
 }
 
 // fp32 partial rows of the largest call of at most that many pairs and chunks
 // (a row of every query head per split), so that a workspace made for the
 // largest batch serves smaller ones, which have more splits each.
 size_t adm_part_bytes(long long pairs, int group, int max_chunks) {
-  const long long deepest = (max_chunks + kAdmMaxCps - 1) / kAdmMaxCps;
+  const long long deepest = (max_chunks + kAdmMaxCps / 2 - 1) / (kAdmMaxCps / 2);
   const long long most = std::max(1, (int)(std::sqrt((double)max_chunks) / 2));
   const long long parts = std::max(pairs * deepest, std::min<long long>(device_sm_count(), pairs * most));
   return (size_t)parts * group * kAdmRowFloats * 4;
