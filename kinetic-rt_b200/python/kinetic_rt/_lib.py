@@ -471,18 +471,24 @@ def _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_h
         raise ValueError(f"{who}: kv_pool must be contiguous and hold num_blocks blocks")
 
 
+_torch_c = None
+
+
 def _launch(who, fn, args, stream):
     """Launches go to the current device, where the tensors must live, on its
     current stream or the given one (a handle, as for the other calls).  A
     decode loop pays for every call, so the struct's byref and its device index
-    are kept with it and the stream is read as a raw handle."""
-    import torch
-    device = torch._C._cuda_getDevice()
+    are kept with it, torch's bindings are looked up once and the stream is
+    read as a raw handle."""
+    global _torch_c
+    if _torch_c is None:
+        import torch
+        _torch_c = torch._C
+    device = _torch_c._cuda_getDevice()
     if device != args._index:
         raise ValueError(f"{who}: the tensors are on cuda:{args._index}, the current device is cuda:{device} "
                          "(torch.cuda.set_device)")
-    stream = torch._C._cuda_getCurrentRawStream(device) if stream is None else int(stream)
-    rc = fn(args._ref, stream)
+    rc = fn(args._ref, _torch_c._cuda_getCurrentRawStream(device) if stream is None else int(stream))
     if rc != KRT_OK:
         check(rc)
 
