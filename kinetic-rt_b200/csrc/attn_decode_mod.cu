@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
   uint8_t* wstage = smem + (size_t)warp * kAdmStages * kAdmStageBytes;
   const uint32_t wstage_u32 = smem_u32(wstage);
   // lane 0 issues this warp's loads: the k-th chunk of the warp is
-  // warp + 4 k of the CTA's and uses stage k % 3
+  // warp + kAdmWarps * k of the CTA's and uses stage k % kAdmStages
   auto issue = [&](int k) {
     const int tok = tl->tok[warp + kAdmWarps * k];
     uint64_t* bar = &tl->full[warp][k % kAdmStages];
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
         mma_bf16_16816(o[2 * jj + 1], pa, bf[2], bf[3]);
       }
     }
-    // ---- refill the stage with this warp's chunk k + 3
+    // ---- refill the stage with this warp's chunk k + kAdmStages
     __syncwarp();
     if (k + kAdmStages < my_chunks) {
       if (lane == 0) {
