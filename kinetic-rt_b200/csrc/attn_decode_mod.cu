@@ -14,17 +14,19 @@
 // swizzled; 192 KB under way per SM); Q K^T and P V on mma.sync m16n8k16 with
 // the group's query heads in the rows (about 4 FLOP a byte: the tensor rate
 // does not matter), statistics and sums in fp32; P is rounded to bf16 for P V
-// (relative 2^-9, as V is).  Warps merge in shared memory, splits in the
-// workspace by the last CTA to finish, in split order, so results do not
-// depend on which CTA that is.  Measured: 128 sequences of 4224 tokens, 8 KV
-// heads (2.2 GB) in 321 us = 6.9 TB/s; one sequence of 4224 tokens 11.1 us in
-// a graph, of which 5 are a CTA's start, its two merges and the launch.
+// (relative 2^-9, as V is).  Warps merge in shared memory; splits through the
+// shared memory of a cluster, or in the workspace by the last CTA to finish;
+// always in split order, so results do not depend on which CTA that is.
+// Measured: 128 sequences of 4224 tokens, 8 KV heads (2.2 GB) in 321 us =
+// 6.9 TB/s; one sequence of 4224 tokens 9.0 us in a graph, of which about 5 are
+// the launch, a CTA's start and its merges.
 //
 // V rows of tokens that are not visible are set to zero in shared memory
 // before P V: their weight is 0, and 0 * inf or 0 * NaN from a cache slot
 // nothing was written to would spoil the row.  Only the first and last chunk
 // of the visible range hold such tokens.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -45,6 +47,7 @@ constexpr int kAdmChunk = 16;               // tokens per TMA box
 constexpr uint32_t kAdmStageBytes = 8192;   // K and V of 16 tokens, one KV head
 constexpr int kAdmMaxGroup = 16;            // query heads per KV head
 constexpr int kAdmRowFloats = 4 + kHeadDim; // max, sum, (two unused), 128 outputs
+constexpr int kAdmMaxCluster = 8;           // splits that merge through shared memory at most
 constexpr int kAdmMaxCps = 1024;            // 16-token chunks per CTA at most
 
 struct AdmParams {
@@ -61,6 +64,7 @@ struct AdmParams {
   int n_kv_heads, group;
   int q_stride, out_stride, lse_stride;
   int chunks_per_split, max_splits;
+  int cluster;               // the splits of a (sequence, KV head) are one cluster
   int max_len;
   ScoreMod mod;
 };
@@ -328,7 +332,10 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
   __syncthreads();
   // thread -> (row, 8 dims) pairs of the merged result
   const bool single = splits == 1;
-  float* part = p.part + (((size_t)b * p.n_kv_heads + kvh) * p.max_splits + z) * (size_t)G * kAdmRowFloats;
+  // this CTA's merged rows: behind the warps' rows, or in the workspace
+  float* mine = wrow + WARPS * kAdmMaxGroup * kAdmRowFloats;
+  float* part = p.cluster ? mine
+                          : p.part + (((size_t)b * p.n_kv_heads + kvh) * p.max_splits + z) * (size_t)G * kAdmRowFloats;
   for (int idx = threadIdx.x; idx < G * 16; idx += kAdmThreads) {
     const int row = idx >> 4, d0 = (idx & 15) * 8;
     float M = -INFINITY;
@@ -357,24 +364,10 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
   }
   if (single) return;
 
-  // ---- several splits: the last CTA of this (sequence, KV head) merges them
-  __threadfence();  // this CTA's partial is visible GPU-wide before the count
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    uint32_t* ctr = p.counters_end - 1 - ((size_t)b * p.n_kv_heads + kvh);
-    const uint32_t prev = atomicAdd(ctr, 1u);
-    const bool last = prev + 1 == (uint32_t)splits;
-    if (last) *ctr = 0u;  // ready for the next call
-    tl->last = last ? 1 : 0;
-  }
-  __syncthreads();
-  if (!tl->last) return;
-  __threadfence();
-  const float* base = p.part + ((size_t)b * p.n_kv_heads + kvh) * p.max_splits * (size_t)G * kAdmRowFloats;
-  for (int idx = threadIdx.x; idx < G * 16; idx += kAdmThreads) {
-    const int row = idx >> 4, d0 = (idx & 15) * 8;
-    // splits in groups whose loads are all under way together: each round
-    // trip to the L2 is about a third of a short call's whole time
+  // ---- several splits, merged in their order.  at(k, i): four floats of split
+  // k's rows from float i; in groups whose loads are all under way together
+  auto join = [&](int idx, auto&& at) {
+    const int row = idx >> 4, d0 = (idx & 15) * 8, first = row * kAdmRowFloats;
     float M = -INFINITY, L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int z0 = 0; z0 < splits; z0 += 8) {
       float m[8], ls[8];
@@ -382,11 +375,12 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const bool in = z0 + k < splits;
-        const float* src = base + ((size_t)(in ? z0 + k : z0) * G + row) * kAdmRowFloats;
-        m[k] = in ? __ldcg(src) : -INFINITY;
-        ls[k] = in ? __ldcg(src + 1) : 0.f;
-        lo4[k] = __ldcg(reinterpret_cast<const float4*>(src + 4 + d0));
-        hi4[k] = __ldcg(reinterpret_cast<const float4*>(src + 8 + d0));
+        const int zz = in ? z0 + k : z0;
+        const float4 ml = at(zz, first);
+        m[k] = in ? ml.x : -INFINITY;
+        ls[k] = in ? ml.y : 0.f;
+        lo4[k] = at(zz, first + 4 + d0);
+        hi4[k] = at(zz, first + 8 + d0);
       }
       float mx = M;
 #pragma unroll
@@ -413,7 +407,36 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
       }
     }
     adm_write_row(p, b, kvh * G + row, d0, acc, M, L);
+  };
+  if (p.cluster) {
+    // the splits are the CTAs of a cluster (those beyond `splits` have left):
+    // each reads its share of the rows from the others' shared memory
+    cluster_sync();
+    const uint32_t rows = smem_u32(mine);
+    const int idx = z + splits * threadIdx.x;
+    if (idx < G * 16)
+      join(idx, [&](int k, int i) { return ld_cluster_f4(map_smem_to_rank(rows, (uint32_t)k) + 4u * (uint32_t)i); });
+    cluster_sync();  // no CTA leaves while its rows are read
+    return;
   }
+  // through the workspace: the last CTA of this (sequence, KV head) merges
+  __threadfence();  // this CTA's partial is visible GPU-wide before the count
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t* ctr = p.counters_end - 1 - ((size_t)b * p.n_kv_heads + kvh);
+    const uint32_t prev = atomicAdd(ctr, 1u);
+    const bool last = prev + 1 == (uint32_t)splits;
+    if (last) *ctr = 0u;  // ready for the next call
+    tl->last = last ? 1 : 0;
+  }
+  __syncthreads();
+  if (!tl->last) return;
+  __threadfence();
+  const float* base = p.part + ((size_t)b * p.n_kv_heads + kvh) * p.max_splits * (size_t)G * kAdmRowFloats;
+  for (int idx = threadIdx.x; idx < G * 16; idx += kAdmThreads)
+    join(idx, [&](int k, int i) {
+      return __ldcg(reinterpret_cast<const float4*>(base + (size_t)k * G * kAdmRowFloats + i));
+    });
 }
 
 typedef void (*AdmKernel)(const CUtensorMap, const AdmParams);
@@ -445,8 +468,8 @@ int adm_max_chunks(int max_seq_len, int window) {
 // CTAs per (sequence, KV head): as many as fill the SMs once, but at most
 // sqrt(chunks) / 2 (the merge grows with their number as the scan shrinks).
 // More, smaller pieces lose: every CTA starts its pipeline, merges its warps
-// and leaves an fp32 partial.  Measured (us), pairs x chunks, this rule against
-// two CTAs per SM and more: 256 x 65 25.6 : 31.0, 160 x 63 17.5 : 25.6,
+// and leaves an fp32 partial.  Measured (us, merged through the workspace),
+// pairs x chunks, this rule against two CTAs per SM and more: 256 x 65 25.6 : 31.0, 160 x 63 17.5 : 25.6,
 // 128 x 128 26.0 : 31.7, 8 x 512 14.7 : 17.1 (37 splits 26.8),
 // 8 x 264 11.1 : 17.5.  Long scans that leave a tenth of the SMs idle are cut
 // at 512 chunks, which evens out ragged lengths: 40 x 4096 177 : 190,
@@ -457,6 +480,35 @@ int adm_splits(long long pairs, int max_chunks) {
   const long long s = std::max(1ll, std::min(sms / pairs, most));
   const int deepest = 10 * s * pairs >= 9 * sms && s * pairs <= sms ? kAdmMaxCps : kAdmMaxCps / 2;
   return (int)std::max<long long>(s, (max_chunks + deepest - 1) / deepest);
+}
+
+// Clusters of `size` CTAs of eight warps that can be resident at once on the
+// current device (asked once per kernel, size and device).
+int adm_clusters(bool cap, bool bias, int size) {
+  static std::atomic<int> known[16][4][kAdmMaxCluster + 1];  // the count + 1, 0: not asked yet
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::atomic<int>* at = dev < 16 ? &known[dev][2 * cap + bias][size] : nullptr;
+  if (at && (n = at->load(std::memory_order_relaxed)) != 0) return n - 1;
+  AdmKernel kern = adm_kernel<8>(cap, bias);
+  const size_t smem = adm_smem_bytes<8>();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = (unsigned)size;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1, 1, (unsigned)size);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (at) at->store(n + 1, std::memory_order_relaxed);
+  return n;
 }
 
 // fp32 partial rows of the largest call of at most that many pairs and chunks
@@ -538,23 +590,36 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   p.lse_stride = a->lse_stride;
   p.max_len = a->max_seq_len;
   const long long pairs = (long long)a->num_seqs * a->n_kv_heads;
-  const int splits = adm_splits(pairs, max_chunks);
+  const bool cap = a->softcap > 0.f, bias = a->alibi_slopes != nullptr;
+  int splits = adm_splits(pairs, max_chunks);
+  // Splits of one cluster merge through shared memory, 1.3 to 2 us sooner than
+  // through the workspace (1 x 4224 tokens 10.9 : 9.0, 1 x 500 7.1 : 5.9,
+  // 40 pairs x 188 chunks 17.9 : 15.9): as many of them as the clusters that
+  // fit allow, unless the longer scan (90 ns a chunk) costs more than that.
+  for (int c = std::min(splits, kAdmMaxCluster); c > 1; --c) {
+    if ((long long)max_chunks * (splits - c) > 20ll * c * splits) break;
+    if (adm_clusters(cap, bias, c) >= pairs) {
+      splits = c;
+      p.cluster = 1;
+      break;
+    }
+  }
   p.chunks_per_split = (max_chunks + splits - 1) / splits;
   p.max_splits = (max_chunks + p.chunks_per_split - 1) / p.chunks_per_split;
+  if (p.max_splits == 1 || (p.cluster && adm_clusters(cap, bias, p.max_splits) < pairs)) p.cluster = 0;
   if (p.max_splits > 65535) return set_error(KRT_ERR_UNSUPPORTED, "%s: max_seq_len is too long", name);
   p.mod = make_score_mod(a->scale, a->softcap, a->alibi_slopes, a->window);
   CUtensorMap tmap;
   int rc = make_tmap_pool_kv16(&tmap, a->kv_pool, a->num_blocks, a->tokens_per_block, a->n_kv_heads, true);
   if (rc) return rc;
   // Eight warps and one CTA per SM, unless the CTAs are one to two per SM:
-  // then four warps, so that all are resident at once.  Measured (us), eight :
+  // then four warps, so that all are resident at once (clusters fit one per SM).  Measured (us), eight :
   // four: 100 CTAs x 264 chunks 39.7 : 45.1, 75 x 125 16.9 : 23.1,
   // 64 x 33 11.1 : 12.6; 160 x 63 23.2 : 17.5, 256 x 65 28.4 : 25.6;
   // 320 x 128 61.6 : 68.5, 320 x 264 117 : 136, 1024 x 264 325 : 322.
   const long long ctas = pairs * p.max_splits;
   const bool eight = ctas <= device_sm_count() || ctas > 2 * device_sm_count();
-  AdmKernel kern = eight ? adm_kernel<8>(a->softcap > 0.f, a->alibi_slopes != nullptr)
-                         : adm_kernel<4>(a->softcap > 0.f, a->alibi_slopes != nullptr);
+  AdmKernel kern = eight ? adm_kernel<8>(cap, bias) : adm_kernel<4>(cap, bias);
   const size_t smem = eight ? adm_smem_bytes<8>() : adm_smem_bytes<4>();
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_error(e, name);
@@ -563,11 +628,15 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   cfg.blockDim = dim3(eight ? 256 : 128, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = (unsigned)p.max_splits;
+  if (p.cluster) cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, kern, tmap, p);
   if (e != cudaSuccess) return cuda_error(e, name);
   return clear_error();

@@ -474,6 +474,12 @@ __device__ __forceinline__ void cluster_arrive_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+// All threads of the cluster's running CTAs; shared memory written before it
+// is seen by the others after it.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // Bulk copy of `bytes` (multiple of 16, 16-byte aligned ends) from this
 // CTA's shared memory to shared memory of another CTA of the cluster; the
 // transfer completes `bytes` of transaction count on the mbarrier at
@@ -495,6 +501,16 @@ __device__ __forceinline__ uint32_t map_smem_to_rank(uint32_t smem_addr, uint32_
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
   return r;
+}
+
+// 16 bytes of another CTA's shared memory (an address of map_smem_to_rank).
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 // ------------------------------------------------------- cross-GPU flags
