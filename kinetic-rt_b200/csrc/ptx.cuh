@@ -314,7 +314,9 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
 
 // High word of it, and the low word (LBO unused).
 constexpr uint32_t kUmmaDescHiSw128 = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t smem_addr) { return ((smem_addr >> 4) & 0x3FFF) | (1u << 16); }
+__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t smem_addr) {
+  return ((smem_addr >> 4) & 0x3FFF) | (1u << 16);
+}
 // Low word for an MN-major operand (128-byte swizzle, same high word): a row of
 // 128 bytes is one k and 64 consecutive m or n; 8-row (k) groups lie 1024 bytes
 // apart (SBO), the next 64 m or n start `mn_stride` bytes on (LBO).

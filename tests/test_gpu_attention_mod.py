@@ -479,3 +479,48 @@ def test_prefill_many_sequences(torch_cuda):
     c = Case(torch_cuda, [int(n) for n in rng.integers(0, 60, 300)], q_lens=q_lens, n_heads=4, n_kv_heads=2, seed=41,
              rows_pad=3)
     c.check(softcap=30.0)
+
+
+def test_calls_at_once(torch_cuda):
+    """Prompt, split prompt and decode calls on three streams at the same time, each with its own workspace."""
+    torch = torch_cuda
+    cases = [Case(torch, [0, 0], q_lens=[900, 700], seed=42), Case(torch, [6000], q_lens=[9], seed=43),
+             Case(torch, [3000, 20, 900], seed=44)]
+    args = [c.args(softcap=30.0) for c in cases]
+    alone = []
+    for c, a in zip(cases, args):
+        c.launch(a)
+        torch.cuda.synchronize()
+        alone.append((c.out.clone(), c.lse.clone()))
+        c.out.fill_(9.0)
+        c.lse.fill_(7.0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        for c, a, s in zip(cases, args, streams):
+            with torch.cuda.stream(s):
+                c.launch(a)
+    torch.cuda.synchronize()
+    for c, (out, lse) in zip(cases, alone):
+        assert torch.equal(c.out, out) and torch.equal(c.lse, lse)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_blocks_far_into_a_large_pool(torch_cuda, prompt):
+    """Blocks more than 2^32 bytes into the pool give what the same blocks give at its start."""
+    torch = torch_cuda
+    near = Case(torch, [700, 90], q_lens=[70, 5] if prompt else None, n_heads=8, n_kv_heads=8, seed=45)
+    a = near.args(softcap=30.0)
+    near.launch(a)
+    torch.cuda.synchronize()
+    want = near.out.clone(), near.lse.clone()
+    far = (9 << 29) // (near.tpb * 2 * 8 * 256)  # 4.5 GiB of blocks before them
+    pool = torch.empty((far + near.blocks,) + tuple(near.pool_d.shape[1:]), dtype=torch.bfloat16, device="cuda")
+    pool[far:].copy_(near.pool_d)
+    near.pool_d, near.blocks = pool, far + near.blocks
+    near.table_d += far
+    near.out.fill_(9.0)
+    near.lse.fill_(7.0)
+    near.launch(near.args(softcap=30.0))
+    torch.cuda.synchronize()
+    assert torch.equal(near.out, want[0]) and torch.equal(near.lse, want[1])

@@ -158,3 +158,27 @@ def test_side_stream_and_graph(torch_cuda):
         g.replay()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(q_out, want[0]) and torch.equal(pool, want[1])
+
+
+def test_blocks_far_into_a_large_pool(torch_cuda):
+    """A slot more than 2^32 bytes into the pool; the slots around it stay as they were."""
+    torch = torch_cuda
+    from python.kinetic_rt import _lib
+    H, K, tpb = 4, 8, 16
+    far = (9 << 29) // (tpb * 2 * K * 256)  # 4.5 GiB of blocks before the used ones
+    pool = torch.empty(far + 2, tpb, 2, K, 128, dtype=torch.bfloat16, device="cuda")
+    pool[far:] = 7.0
+    x = torch.randn(3, (H + 2 * K) * 128, device="cuda").to(torch.bfloat16)
+    q_out = torch.zeros(3, H * 128, dtype=torch.bfloat16, device="cuda")
+    ws = torch.zeros(_lib.rope_append_workspace_bytes(), dtype=torch.uint8, device="cuda")
+    pos = torch.tensor([0, 17, 31], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[far + 1, far]], dtype=torch.int32, device="cuda")
+    f = 0.5 ** torch.arange(64, dtype=torch.float64, device="cuda")
+    _lib.rope_append(_lib.rope_append_args(x[:, :H * 128], x[:, H * 128:(H + K) * 128], x[:, (H + K) * 128:], f, pos,
+                                           torch.zeros_like(pos), table, pool, q_out, H, K, far + 2, tpb, ws))
+    assert _lib.read_status(ws) == (0, 0)
+    got = pool[far:, :, 1]
+    want = torch.full_like(got, 7.0)
+    for t, (b, o) in enumerate(((1, 0), (0, 1), (0, 15))):
+        want[b, o] = x[t, (H + K) * 128:].view(K, 128)
+    assert torch.equal(got, want)
