@@ -44,7 +44,7 @@
 // slots (the cap's polynomial, maxima, packing) come on top of what the
 // special-function units leave of them.  Measured: six chunks of 517 tokens
 // behind 3700, 64 heads, 296 us = 957 TFLOP/s; 8 x 2048, 32 heads, causal,
-// capped, 357 us = 770 TFLOP/s; 64 tokens alone, 9.4 us in a graph.
+// capped, 357 us = 770 TFLOP/s; 64 tokens alone, 9.9 us in a graph.
 // Steps that are spared:
 //   * the reference that scores are taken against is the row's old maximum
 //     unless it grew by more than 2^16 (weights then stay below that, and bf16
