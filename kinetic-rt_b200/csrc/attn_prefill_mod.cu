@@ -36,6 +36,8 @@
 // sums a second kernel joins.  Measured, 8 tokens of 8 KV heads behind 65536:
 // 726 us whole, 64 split; behind 8192: 100 and 25; behind 1024: 19 and 17.
 // (Pieces of four blocks: 14 there, but a 512-token prompt takes 20 for 17.)
+// The last items of a long causal prompt are split too where the others would
+// end well before them.
 //
 // What bounds it: per 128 keys and pair of tiles the tensor core needs about
 // 2560 cycles (2048 of arithmetic; at N = 64 Q K^T reads 6 KB of shared memory
@@ -50,6 +52,9 @@
 //     unless it grew by more than 2^16 (weights then stay below that, and bf16
 //     and the fp32 sum lose nothing by it); only then O and the sum are
 //     rescaled, after the tile's last P V;
+//   * under a distance bias blocks are taken from the last to the first: the
+//     nearest keys then set the reference, where in ascending order it would
+//     grow with every block (documents with a bias: 171 us, ascending 199);
 //   * the cap is a polynomial of the score while scores are well below it, and
 //     its value at the row's largest |score| serves as the reference.
 //
@@ -108,6 +113,7 @@ struct ApmParams {
   int* status;
   uint32_t* queue;           // [next piece, CTAs that are through], zero between launches
   int items, splits;         // items, and pieces of each, at most
+  int piece;                 // key blocks of a piece
   float4* part_o;            // [piece][tile][column / 4][row]
   float2* part_ml;           // [piece][tile][row] reference and sum
   int32_t* part_flags;       // [piece][tile] V values that are not finite were taken out
@@ -278,7 +284,7 @@ __device__ __forceinline__ ApmItem apm_find(const ApmParams& p, int index, int l
 // Key blocks per piece of the item, and how many pieces that makes.
 __device__ __forceinline__ int apm_pieces(const ApmParams& p, const ApmItem& it, int* len) {
   const int blocks = (it.hi_all + kApmBlock - 1) / kApmBlock - it.lo_all / kApmBlock;
-  *len = max(kApmMinPiece, (blocks + p.splits - 1) / p.splits);
+  *len = max(p.piece, (blocks + p.splits - 1) / p.splits);
   return max(1, (blocks + *len - 1) / *len);
 }
 
@@ -448,14 +454,14 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       }
       const int g0 = it.lo_all / kApmBlock, g1 = (it.hi_all + kApmBlock - 1) / kApmBlock;
       const int32_t* table = p.block_table + (size_t)it.seq * p.bt_stride;
-      // pool token of this lane's page of block g (lanes 0-3), -1 where the lookup failed
-      auto look_up = [&](int g) {
-        const int j = g * kApmBlock + (lane & 3) * kApmPage;
+      // pool token of this lane's page of step o's block (lanes 0-3), -1 where the lookup failed
+      auto look_up = [&](int o) {
+        const int j = (BIAS ? g1 - 1 - o : g0 + o) * kApmBlock + (lane & 3) * kApmPage;
         int v = outside;
-        if (g < g1 && j < it.hi_all && j + kApmPage > it.lo_all) v = (int)apm_slot(p, table, j);
+        if (o < g1 - g0 && j < it.hi_all && j + kApmPage > it.lo_all) v = (int)apm_slot(p, table, j);
         return v;
       };
-      int pool_tok = look_up(g0), next_tok = look_up(g0 + 1);
+      int pool_tok = look_up(0), next_tok = look_up(1);
       if (kv == 0 && g1 > g0) {
         if (q_count > 0 && !mbar_wait_all(&tl->q_empty, (uint32_t)(q_count - 1) & 1u, abort_flag)) {
           if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
@@ -473,14 +479,14 @@ __global__ void __launch_bounds__(kApmThreads, 1)
         __syncwarp();
       }
 #pragma unroll 1
-      for (int g = g0; g < g1; ++g) {
+      for (int o = 0; o < g1 - g0; ++o) {
         const uint32_t bad = __ballot_sync(0xffffffffu, pool_tok < 0) & 15u;
         if (pool_tok < 0) pool_tok = outside;
         int page[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) page[c] = __shfl_sync(0xffffffffu, pool_tok, c);
         pool_tok = next_tok;
-        next_tok = look_up(g + 2);  // two blocks ahead: the lookup is not waited for
+        next_tok = look_up(o + 2);  // two blocks ahead: the lookup is not waited for
         if (count >= kApmStages && !mbar_wait_all(&tl->empty[kv][slot], ph ^ 1u, abort_flag)) {
           if (lane == 0) apm_fail(p, tl, kStatusTimeoutEmpty);
           ok = false;
@@ -534,11 +540,14 @@ __global__ void __launch_bounds__(kApmThreads, 1)
         break;
       }
       const int seq = at->seq, g0 = at->lo_all / kApmBlock, g1 = (at->hi_all + kApmBlock - 1) / kApmBlock;
-      // (a tile without a live row has no blocks in any step)
-      const int t_end = at->end[i], t_begin = t_end == 0 ? g1 : at->first[i];
+      const int steps = g1 - g0;
+      // steps in which the tile takes part (one without a live row: in none)
+      const bool any = at->end[i] > 0;
+      const int t_begin = !any ? steps : BIAS ? g1 - at->end[i] : at->first[i] - g0;
+      const int t_end = !any ? 0 : t_begin + at->end[i] - at->first[i];
       release_item(k);
       if (seq < 0) break;
-      if (g1 <= g0) continue;
+      if (steps <= 0) continue;
       if (!mbar_wait_all(&tl->q_full, (uint32_t)q_count & 1u, abort_flag)) {
         if (lane == 0) apm_fail(p, tl, kStatusTimeoutFull);
         ok = false;
@@ -546,10 +555,10 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       }
       ++q_count;
 #pragma unroll 1
-      for (int g = g0 - 2; g < g1; ++g) {
+      for (int g = -2; g < steps; ++g) {
         const int b = g - t_begin;             // the item's how-manieth block of the tile
         const uint32_t n = (uint32_t)(done + b);  // of all items; its buffer is n & 1
-        const bool has_k = g + 2 < g1, has_v = g >= g0;
+        const bool has_k = g + 2 < steps, has_v = g >= 0;
         if (has_k) ok = mbar_wait_all(&tl->full[0][k_slot], k_ph, abort_flag);
         if (has_v && ok) ok = mbar_wait_all(&tl->full[1][v_slot], v_ph, abort_flag);
         if (!ok) {
@@ -590,7 +599,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
         if (leader) {
           if (has_v) umma_commit(&tl->empty[1][v_slot]);
           if (has_k) umma_commit(&tl->empty[0][k_slot]);
-          if (g + 3 == g1) umma_commit(&tl->q_empty);  // the item's last Q K^T
+          if (g + 3 == steps) umma_commit(&tl->q_empty);  // the item's last Q K^T
         }
         __syncwarp();
         if (has_v && ++v_slot == kApmStages) {
@@ -643,7 +652,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       }
       const int w_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0);        // keys that all live rows of the
       const int w_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);  // warp see
-      const int g0 = at->lo_all / kApmBlock;
+      const int g0 = at->lo_all / kApmBlock, g1 = (at->hi_all + kApmBlock - 1) / kApmBlock;
       float m_ref = -INFINITY, l = 0.f;
       float slope2 = 0.f;
       if (BIAS && valid) slope2 = p.mod.slopes[at->kvh * G + r - row_tok * G] * 1.4426950408889634f;
@@ -656,11 +665,11 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           break;
         }
         tc_fence_after();
-        const int g = first + b, j0 = g * kApmBlock;
+        const int g = BIAS ? first + n - 1 - b : first + b, j0 = g * kApmBlock;
         float x[64];
         tmem_ld32_nowait(s_addr, x);
         tmem_ld32_nowait(s_addr + 32, x + 32);
-        const int m = blocks + g - g0;  // of the CTA's blocks
+        const int m = blocks + (BIAS ? g1 - 1 - g : g - g0);  // of the CTA's blocks
         const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&tl->bad[m & 15]);
         const bool masked = j0 < w_lo || j0 + kApmBlock > w_hi || bad != 0;  // for some live row of the warp
         if (j0 < at->lo_max || j0 + kApmBlock > at->hi_min) {
@@ -894,7 +903,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
               !live || l == 0.f ? -INFINITY : (m_ref == -INFINITY ? l : (m_ref + log2f(l)) * kLn2);
       }
       done += n;
-      blocks += (at->hi_all + kApmBlock - 1) / kApmBlock - g0;
+      blocks += g1 - g0;
       release_item(k);
     }
     if (!ok && lane == 0) apm_fail(p, tl, kStatusTimeoutAccum);
@@ -995,7 +1004,7 @@ long long apm_items(int num_tokens, int num_seqs, int n_heads, int n_kv_heads) {
   return (num_tokens / (2 * tile_tokens) + (long long)num_seqs) * n_kv_heads;
 }
 
-int apm_max_pieces() { return std::min(device_sm_count(), kApmMaxPieces); }
+int apm_max_pieces() { return std::min(3 * device_sm_count(), kApmMaxPieces); }
 
 // Pieces that an item of so many key blocks is worth at most.
 long long apm_worth(long long blocks) { return (blocks + kApmMinPiece - 1) / kApmMinPiece; }
@@ -1078,11 +1087,25 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   p.mod = make_score_mod(a->scale, a->softcap, a->alibi_slopes, a->window);
   const long long items = apm_items(a->num_tokens, a->num_seqs, a->n_heads, a->n_kv_heads), sms = device_sm_count();
   if (items > INT_MAX) return set_error(KRT_ERR_UNSUPPORTED, "%s: too many tokens or heads", name);
-  // Few rows before a long cache: their keys are split so that all SMs work.
-  long long blocks = apm_blocks(a->max_kv_len);
-  if (a->window > 0) blocks = std::min(blocks, apm_blocks((long long)a->window + 2 * p.tile_tokens) + 1);
+  // Few rows behind a long cache: items are split so that all SMs work.  Else
+  // items that are longer than an SM's share of all by far are, so that none
+  // ends late: the last rows of a long causal prompt (half a prompt's own keys
+  // lie behind its average row; lengths are taken as equal).  4096 tokens of 8
+  // heads on one KV head: 72 us whole, 57 split.
+  long long longest = apm_blocks(a->max_kv_len), average = longest;
+  if (a->window > 0)
+    average = longest = std::min(longest, apm_blocks((long long)a->window + 2 * p.tile_tokens) + 1);
+  else
+    average = std::max(longest / 2, longest - apm_blocks(a->num_tokens / a->num_seqs) / 2);
+  long long splits = std::min(sms / items, apm_worth(longest)), piece = kApmMinPiece;
+  const long long share = (items * average + sms - 1) / sms;
+  if (2 * items > sms && longest - share >= 20) {
+    splits = std::min(apm_max_pieces() / items, (longest + share - 1) / share);
+    piece = share;
+  }
   p.items = (int)items;
-  p.splits = (int)std::max(1ll, std::min(apm_max_pieces() / items, apm_worth(blocks)));
+  p.splits = (int)std::max(1ll, splits);
+  p.piece = (int)std::max(piece, (longest + p.splits - 1) / p.splits);
   p.part_ml = reinterpret_cast<float2*>(ws + kWsHeaderBytes);
   p.part_o = reinterpret_cast<float4*>(ws + kWsHeaderBytes + (size_t)items * p.splits * kApmStatBytes);
   CUtensorMap tmap_q, tmap_kv;

@@ -524,3 +524,13 @@ def test_blocks_far_into_a_large_pool(torch_cuda, prompt):
     near.launch(near.args(softcap=30.0))
     torch.cuda.synchronize()
     assert torch.equal(near.out, want[0]) and torch.equal(near.lse, want[1])
+
+
+def test_prefill_long_causal_items_are_split(torch_cuda):
+    """A long prompt of one KV head: its last items are in pieces, its first whole; ascending and (bias) descending."""
+    n = 4100
+    c = Case(torch_cuda, [0], q_lens=[n], n_heads=8, n_kv_heads=1, seed=46)
+    only = set(range(5, n, 211)) | {0, n - 1}
+    c.check(only=only)
+    c.check(only=only, slopes=slopes_of(8))
+    c.check(only=only, slopes=slopes_of(8), softcap=30.0, prefix=[2000])
