@@ -8,7 +8,7 @@
 //
 // Every visible K/V byte is read once, so the kernel is bound by HBM; the
 // invisible ones (before the window or the document) are not read.  Grid
-// (sequence, KV head, split of the visible 16-token chunks); four or eight
+// (sequence, KV head, split of the visible 16-token chunks); two, four or eight
 // warps take the CTA's chunks in turn, each with its own ring of three 8 KB
 // stages (one 5-D TMA box = K and V of 16 tokens of one KV head, 128-byte
 // swizzled; 192 KB under way per SM); Q K^T and P V on mma.sync m16n8k16 with
@@ -612,20 +612,24 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   CUtensorMap tmap;
   int rc = make_tmap_pool_kv16(&tmap, a->kv_pool, a->num_blocks, a->tokens_per_block, a->n_kv_heads, true);
   if (rc) return rc;
-  // Eight warps and one CTA per SM, unless the CTAs are one to two per SM:
-  // then four warps, so that all are resident at once (clusters fit one per SM).  Measured (us), eight :
-  // four: 100 CTAs x 264 chunks 39.7 : 45.1, 75 x 125 16.9 : 23.1,
-  // 64 x 33 11.1 : 12.6; 160 x 63 23.2 : 17.5, 256 x 65 28.4 : 25.6;
-  // 320 x 128 61.6 : 68.5, 320 x 264 117 : 136, 1024 x 264 325 : 322.
-  const long long ctas = pairs * p.max_splits;
-  const bool eight = ctas <= device_sm_count() || ctas > 2 * device_sm_count();
-  AdmKernel kern = eight ? adm_kernel<8>(cap, bias) : adm_kernel<4>(cap, bias);
-  const size_t smem = eight ? adm_smem_bytes<8>() : adm_smem_bytes<4>();
+  // Eight warps and one CTA per SM, or four and two CTAs, so that all are
+  // resident at once (clusters fit one per SM).  Of more CTAs than that, short
+  // ones take two warps, four per SM: their start and end dominate.  Measured
+  // (us), eight : four : two warps: 100 CTAs x 264 chunks 39.7 : 45.1,
+  // 75 x 125 16.9 : 23.1; 160 x 63 23.2 : 17.5, 256 x 65 28.4 : 25.6;
+  // 1600 x 1 33 : 18 : 10, 1600 x 32 78 : 70 : 67, 480 x 63 49 : 43 : 42;
+  // ragged 512 x 264 127 : 133 : 139, 1024 x 264 245 : 251 : 265.
+  const long long ctas = pairs * p.max_splits, sms = device_sm_count();
+  const int warps = ctas <= sms ? 8 : ctas <= 2 * sms ? 4 : p.chunks_per_split <= 64 ? 2 : 8;
+  AdmKernel kern = warps == 8   ? adm_kernel<8>(cap, bias)
+                   : warps == 4 ? adm_kernel<4>(cap, bias)
+                                : adm_kernel<2>(cap, bias);
+  const size_t smem = warps == 8 ? adm_smem_bytes<8>() : warps == 4 ? adm_smem_bytes<4>() : adm_smem_bytes<2>();
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_error(e, name);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a->num_seqs, (unsigned)a->n_kv_heads, (unsigned)p.max_splits);
-  cfg.blockDim = dim3(eight ? 256 : 128, 1, 1);
+  cfg.blockDim = dim3(32u * warps, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[2];

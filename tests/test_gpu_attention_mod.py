@@ -534,3 +534,13 @@ def test_prefill_long_causal_items_are_split(torch_cuda):
     c.check(only=only)
     c.check(only=only, slopes=slopes_of(8))
     c.check(only=only, slopes=slopes_of(8), softcap=30.0, prefix=[2000])
+
+
+@pytest.mark.parametrize("seqs,ctx,H,K", [(60, 40, 8, 8), (320, 17, 5, 1), (45, 900, 16, 8), (170, 300, 2, 2)])
+def test_decode_many_short_sequences(torch_cuda, seqs, ctx, H, K):
+    """More CTAs than two per SM, with few chunks each; empty sequences and single tokens among them."""
+    rng = np.random.Generator(np.random.PCG64(seqs))
+    lens = [int(n) for n in rng.integers(0, ctx + 1, seqs)]
+    lens[:3] = [ctx, 1, 0]
+    c = Case(torch_cuda, lens, n_heads=H, n_kv_heads=K, seed=47)
+    c.check(softcap=20.0, slopes=slopes_of(H), only=set(range(0, seqs, 7)) | {1, 2})
