@@ -7,25 +7,24 @@
 // dims R .. 127 pass through.  q goes to q_out, k and v to the slot of the
 // token's cache index (token layout [K | V][kv_head][128] bf16).
 //
-// The kernel reads and writes every element once and is bound by HBM.  A warp
-// takes a token (a CTA of eight warps when there are few tokens): its threads
-// ask for their first vectors, then compute the token's R / 2 cosines and
-// sines into shared memory while those are under way; all heads share them.
-// The angle is taken in fp64 turns (p * inv_freq / 2 pi) and reduced to its
-// fraction before the fp32 sine: at position 10^6 an fp32 angle would be off
-// by 0.06.  This costs R / 2 fp64 products a token, against R * heads products,
-// and saves the table that limits the position.  Unit u of a head is two
-// 8-element vectors that a thread loads, rotates and stores (16-byte
-// accesses): the two partners of a half-split rotation, or two vectors of
-// interleaved pairs.
+// The kernel reads and writes every element once and is bound by HBM.  One to
+// eight warps take a token: its threads ask for their first vectors, then
+// compute the token's R / 2 cosines and sines into shared memory while those
+// are under way; all heads share them.  The angle is taken in fp64 turns
+// (p * inv_freq / 2 pi) and reduced to its fraction before the fp32 sine: at
+// position 10^6 an fp32 angle would be off by 0.06.  This costs R / 2 fp64
+// products a token, against R * heads products, and saves the table that limits
+// the position.  Unit u of a head is two 8-element vectors that a thread loads,
+// rotates and stores (16-byte accesses): the two partners of a half-split
+// rotation, or two vectors of interleaved pairs.  Halves that end inside a
+// vector go through shared memory.
 //
-// Measured: 16384 tokens of 32 + 8 heads (bf16, 403 MB) in 69 us = 5.9 TB/s;
-// 32 k tokens of 8 + 1 heads (fp32 in, 250 MB) in 47 us = 5.3 TB/s: with ten
+// Measured: 16384 tokens of 32 + 8 heads (bf16, 403 MB) in 67 us = 6.0 TB/s;
+// 32 k tokens of 8 + 1 heads (fp32 in, 250 MB) in 46 us = 5.4 TB/s: with ten
 // heads the angles are a third of a warp's time on its token.  More warps
 // matter more than vectors per thread: two fp32 units per thread (two CTAs per
-// SM fewer) take 52 us, four bf16 units 72 us.  A warp per token instead of a
-// CTA for four tokens with a barrier after the angles: 74 to 69 and 60 to 47.
-// 64 tokens take 3.0 us in a graph.
+// SM fewer) take 52 us, four bf16 units 72 us.  A CTA for four tokens with a
+// barrier after the angles took 74 and 60.  64 tokens take 2.8 us in a graph.
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -88,9 +87,6 @@ struct RaVec<__nv_bfloat16> {
     }
   }
 };
-__device__ __forceinline__ float ra_load1(const float* src) { return *src; }
-__device__ __forceinline__ float ra_load1(const __nv_bfloat16* src) { return __bfloat162float(*src); }
-
 __device__ __forceinline__ void ra_store8(__nv_bfloat16* dst, const float* x) {
   *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
                                               pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
@@ -100,15 +96,16 @@ __device__ __forceinline__ void ra_store8(__nv_bfloat16* dst, const float* x) {
 // halves whole vectors; or with halves that end inside a vector.
 enum { kRaInterleaved = 0, kRaHalves = 1, kRaOddHalves = 2 };
 
-// WARPS warps take a token (one: the CTA holds eight tokens).
+// WARPS warps take a token; a CTA of eight holds 8 / WARPS tokens.
 template <typename T, int MODE, int WARPS>
 __global__ void __launch_bounds__(kRaThreads, 4) rope_append_kernel(const RaParams p) {
   constexpr int kLanes = 32 * WARPS, kRows = kLanes / kRaUnits;  // threads of a token, heads they have at a time
   constexpr int kBatch = RaVec<T>::kBatch;
   __shared__ float2 cs_all[kRaThreads / kLanes][64];  // of pair f at ra_at(f)
+  __shared__ __align__(16) float rows[MODE == kRaOddHalves ? kRaThreads / kRaUnits : 1][kHeadDim + 4];
   const int part = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int t = blockIdx.x * (kRaThreads / kLanes) + part;
-  if (t >= p.num_tokens) return;  // whole warps; with several warps per token the grid is exact
+  if (t >= p.num_tokens) return;  // all of the token's warps
   const int H = p.n_heads, K = p.n_kv_heads, heads = H + 2 * K, half = p.rotary_dim / 2;
   float2* cs = cs_all[part];
   // element j of the eight threads of a head in eight neighbouring words
@@ -164,7 +161,7 @@ __global__ void __launch_bounds__(kRaThreads, 4) rope_append_kernel(const RaPara
   if (WARPS == 1)
     __syncwarp();
   else
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + part), "r"(kLanes) : "memory");  // the token's warps
 
   for (const int last = slot >= 0 ? heads : H; head < last;) {
 #pragma unroll
@@ -205,24 +202,33 @@ __global__ void __launch_bounds__(kRaThreads, 4) rope_append_kernel(const RaPara
           }
         }
       } else if (rot) {
-        // partners do not fall on vectors: fetch each one by itself
-        const T* src = source(h);
+        // partners do not fall on vectors: the head's eight threads exchange them
+        // through shared memory
+        float* row = rows[threadIdx.x / kRaUnits];
+        const uint32_t peers = 0xFFu << (threadIdx.x & 24);
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          *reinterpret_cast<float4*>(row + 8 * u + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+          *reinterpret_cast<float4*>(row + 64 + 8 * u + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+        }
+        __syncwarp(peers);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int dx = 8 * u + j, dy = dx + 64;
           if (dx < p.rotary_dim) {
             const int f = dx < half ? dx : dx - half;
             const float2 w = cs[ra_at(f)];
-            const float o = ra_load1(src + (dx < half ? dx + half : f));
+            const float o = row[dx < half ? dx + half : f];
             x[j] = dx < half ? x[j] * w.x - o * w.y : x[j] * w.x + o * w.y;
           }
           if (dy < p.rotary_dim) {
             const int f = dy < half ? dy : dy - half;
             const float2 w = cs[ra_at(f)];
-            const float o = ra_load1(src + (dy < half ? dy + half : f));
+            const float o = row[dy < half ? dy + half : f];
             y[j] = dy < half ? y[j] * w.x - o * w.y : y[j] * w.x + o * w.y;
           }
         }
+        __syncwarp(peers);
       }
       ra_store8(dst + 8 * (rot ? va : u), x);
       ra_store8(dst + 8 * (rot ? vb : u + 8), y);
@@ -234,9 +240,13 @@ __global__ void __launch_bounds__(kRaThreads, 4) rope_append_kernel(const RaPara
 
 typedef void (*RaKernel)(const RaParams);
 template <typename T, int WARPS>
-RaKernel ra_kernel(const RaParams& p) {
+RaKernel ra_kernel_of(const RaParams& p) {
   if (p.interleaved) return rope_append_kernel<T, kRaInterleaved, WARPS>;
   return p.rotary_dim % 16 == 0 ? rope_append_kernel<T, kRaHalves, WARPS> : rope_append_kernel<T, kRaOddHalves, WARPS>;
+}
+template <typename T>
+RaKernel ra_kernel(const RaParams& p, int warps) {
+  return warps == 1 ? ra_kernel_of<T, 1>(p) : warps == 2 ? ra_kernel_of<T, 2>(p) : ra_kernel_of<T, 8>(p);
 }
 
 }  // namespace krt
@@ -315,10 +325,15 @@ extern "C" int krt_rope_append(const krt_rope_append_args* a, void* stream) {
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
   p.factor = a->factor == 0.f ? 1.f : a->factor;
-  // A CTA per token while that leaves SMs free, then a warp per token.
-  const bool cta_each = a->num_tokens < 8 * device_sm_count();
+  // Eight warps per token while the tokens are few, then two, or one where a
+  // token has little work.  Measured (us), eight : two : one: 40 heads (bf16),
+  // 300 tokens 3.5 : 4.8 : 7.4, 1500 8.8 : 8.4 : 9.8, 16000 87 : 66 : 68;
+  // 9 heads (fp32), 300 2.7 : 3.1 : 3.7, 1500 5.9 : 4.5 : 4.6, 16000 55 : 29 : 25.
+  const int sms = device_sm_count(), heads = a->n_heads + 2 * a->n_kv_heads;
+  const int warps = a->num_tokens < 4 * sms ? 8 : heads >= 32 || a->num_tokens < 16 * sms ? 2 : 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cta_each ? (unsigned)a->num_tokens : ((unsigned)a->num_tokens + 7) / 8, 1, 1);
+  const int per_cta = 8 / warps;
+  cfg.gridDim = dim3(((unsigned)a->num_tokens + per_cta - 1) / per_cta, 1, 1);
   cfg.blockDim = dim3(kRaThreads, 1, 1);
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];
@@ -326,9 +341,7 @@ extern "C" int krt_rope_append(const krt_rope_append_args* a, void* stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  RaKernel kern = dtype == KRT_DTYPE_FLOAT32
-                      ? (cta_each ? ra_kernel<float, 8>(p) : ra_kernel<float, 1>(p))
-                      : (cta_each ? ra_kernel<__nv_bfloat16, 8>(p) : ra_kernel<__nv_bfloat16, 1>(p));
+  RaKernel kern = dtype == KRT_DTYPE_FLOAT32 ? ra_kernel<float>(p, warps) : ra_kernel<__nv_bfloat16>(p, warps);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return cuda_error(e, name);
   return clear_error();

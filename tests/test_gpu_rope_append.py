@@ -182,3 +182,10 @@ def test_blocks_far_into_a_large_pool(torch_cuda):
     for t, (b, o) in enumerate(((1, 0), (0, 1), (0, 15))):
         want[b, o] = x[t, (H + K) * 128:].view(K, 128)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T,H,K,R,interleaved,fp32", [(700, 4, 1, 90, False, False), (700, 30, 2, 128, False, True),
+                                                      (2500, 2, 1, 10, True, False), (2499, 1, 1, 66, False, True)])
+def test_many_tokens(torch_cuda, T, H, K, R, interleaved, fp32):
+    """Two warps and one warp per token, CTAs of several tokens, the last one not full."""
+    run(torch_cuda, T, H, K, R, interleaved, fp32=fp32, seed=T + R, skip=(3, T - 1), lost=(8, 640))
