@@ -113,7 +113,7 @@ struct ApmParams {
   int* status;
   uint32_t* queue;           // [next piece, CTAs that are through], zero between launches
   int items, splits;         // items, and pieces of each, at most
-  int piece;                 // key blocks of a piece
+  int piece;                 // key blocks of a piece at least
   float4* part_o;            // [piece][tile][column / 4][row]
   float2* part_ml;           // [piece][tile][row] reference and sum
   int32_t* part_flags;       // [piece][tile] V values that are not finite were taken out
@@ -1105,7 +1105,7 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   }
   p.items = (int)items;
   p.splits = (int)std::max(1ll, splits);
-  p.piece = (int)std::max(piece, (longest + p.splits - 1) / p.splits);
+  p.piece = (int)piece;  // at least; `splits` of the item's real length otherwise
   p.part_ml = reinterpret_cast<float2*>(ws + kWsHeaderBytes);
   p.part_o = reinterpret_cast<float4*>(ws + kWsHeaderBytes + (size_t)items * p.splits * kApmStatBytes);
   CUtensorMap tmap_q, tmap_kv;

@@ -544,3 +544,14 @@ def test_decode_many_short_sequences(torch_cuda, seqs, ctx, H, K):
     lens[:3] = [ctx, 1, 0]
     c = Case(torch_cuda, lens, n_heads=H, n_kv_heads=K, seed=47)
     c.check(softcap=20.0, slopes=slopes_of(H), only=set(range(0, seqs, 7)) | {1, 2})
+
+
+def test_prefill_short_keys_under_a_large_bound(torch_cuda):
+    """max_kv_len far above the lengths: the split follows the real ones."""
+    c = Case(torch_cuda, [1500, 40], q_lens=[6, 20], seed=48)
+    rows = c.rows()
+    ref, lse, tol, tol_lse = orc.paged_attention_mod(c.q, c.pool, c.table, rows, 8, 2, 16)
+    c.table_d = torch_cuda.cat([c.table_d, torch_cuda.zeros(2, 8192, dtype=torch_cuda.int32, device="cuda")], dim=1)
+    c.launch(c.args(max_len=131072))
+    got, got_lse = c.result()
+    assert (np.abs(got - ref) <= tol).all() and (np.abs(got_lse - lse) <= tol_lse).all()
