@@ -715,7 +715,11 @@ __global__ void __launch_bounds__(kApmThreads, 1)
             a1 = max3(a1, fabsf(x[c + 2]), fabsf(x[c + 3]));
           }
           a0 = fmaxf(a0, a1);
-          const bool small = !__any_sync(0xffffffffu, !(a0 <= p.mod.poly_max));
+          // The form is chosen for the warp, and none of its rows' bits may depend on
+          // what lies beside the sequence: rows that are not live (the next
+          // sequence's, or such as no load fills) have no vote, and in blocks with
+          // invisible keys (unwritten cache slots) both forms give the same bits.
+          const bool small = !__any_sync(0xffffffffu, live && !(a0 <= p.mod.poly_max));
           direct = !BIAS && small && !masked && p.mod.cap2 * 0.605f <= kApmBound;
           if (direct) {
             m_new = cap_at(a0, p.mod.poly);  // a reference no lower than the maximum
@@ -727,7 +731,9 @@ __global__ void __launch_bounds__(kApmThreads, 1)
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < 64; ++c) x[c] = cap_score(x[c], p.mod.cap_in, p.mod.cap2);
+            for (int c = 0; c < 64; ++c)
+              x[c] = fabsf(x[c]) <= p.mod.poly_max ? cap_at(x[c], p.mod.poly)
+                                                   : cap_score(x[c], p.mod.cap_in, p.mod.cap2);
           }
         }
         if (BIAS) {
