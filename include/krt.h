@@ -381,10 +381,10 @@ KRT_API int krt_paged_attention_prefill(const krt_paged_prefill_attention_args* 
  * fewer than 2^31 - 16 tokens.  scale 0 = 1 / sqrt(head_dim); scale, softcap and
  * window must not be negative.  Workspaces are zero-filled once when
  * allocated (and again after a status word with a timeout bit); calls that
- * may overlap on the GPU need workspaces of their own.  A workspace made for
- * the most sequences and the longest max_seq_len, passed whole, serves every
- * smaller call of the same heads and window after one another, captured ones
- * too.
+ * may overlap on the GPU need workspaces of their own.  A workspace that is
+ * large enough for each of them serves calls of both attentions, of any sizes,
+ * heads and windows, one after another, captured ones too (other calls of this
+ * header lay theirs out differently: not those).
  * ---------------------------------------------------------------------- */
 
 /* One query token per sequence, at position p = seq_lens[s] - 1 (its K/V are

@@ -58,7 +58,7 @@ struct AdmParams {
   const int32_t* seq_lens;
   const int32_t* kv_start;   // [num_seqs] or NULL
   float* part;               // [num_seqs][n_kv_heads][max_splits][group][kAdmRowFloats]
-  uint32_t* counters_end;    // counter of (sequence, KV head) i at -1 - i
+  uint32_t* counters;        // [num_seqs][n_kv_heads], zero between calls
   int* status;
   int bt_stride, num_blocks, tokens_per_block;
   int n_kv_heads, group;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
   __threadfence();  // this CTA's partial is visible GPU-wide before the count
   __syncthreads();
   if (threadIdx.x == 0) {
-    uint32_t* ctr = p.counters_end - 1 - ((size_t)b * p.n_kv_heads + kvh);
+    uint32_t* ctr = p.counters + (size_t)b * p.n_kv_heads + kvh;
     const uint32_t prev = atomicAdd(ctr, 1u);
     const bool last = prev + 1 == (uint32_t)splits;
     if (last) *ctr = 0u;  // ready for the next call
@@ -528,8 +528,8 @@ extern "C" size_t krt_paged_attention_mod_workspace_size(int32_t num_seqs, int32
   if (num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || max_seq_len <= 0 || window < 0 || n_heads % n_kv_heads != 0)
     return 0;
   const long long pairs = (long long)num_seqs * n_kv_heads;
-  const size_t counters = ((size_t)pairs * 4 + 255) & ~size_t(255);
-  return kWsHeaderBytes + adm_part_bytes(pairs, n_heads / n_kv_heads, adm_max_chunks(max_seq_len, window)) + counters;
+  const size_t own = pairs > kModCounters ? (size_t)pairs * 4 : 0;
+  return kModPartsAt + adm_part_bytes(pairs, n_heads / n_kv_heads, adm_max_chunks(max_seq_len, window)) + own;
 }
 
 extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args* a, void* stream) {
@@ -576,10 +576,8 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   p.kv_start = a->kv_start;
   char* ws = static_cast<char*>(a->workspace);
   p.status = reinterpret_cast<int*>(ws);
-  // partials from the front, counters from the end: calls of other sizes on
-  // the same workspace never leave a partial where a counter is expected at 0
-  p.part = reinterpret_cast<float*>(ws + kWsHeaderBytes);
-  p.counters_end = reinterpret_cast<uint32_t*>(ws + (a->workspace_bytes & ~size_t(3)));
+  p.part = reinterpret_cast<float*>(ws + kModPartsAt);
+  p.counters = reinterpret_cast<uint32_t*>(ws + kModCountersAt);
   p.bt_stride = a->block_table_stride;
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
@@ -627,6 +625,13 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   const size_t smem = warps == 8 ? adm_smem_bytes<8>() : warps == 4 ? adm_smem_bytes<4>() : adm_smem_bytes<2>();
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_error(e, name);
+  if (pairs > kModCounters && p.max_splits > 1 && !p.cluster) {
+    // more pairs than the workspace has counters for: behind the partials, where
+    // other calls leave anything
+    p.counters = reinterpret_cast<uint32_t*>(ws + kModPartsAt + adm_part_bytes(pairs, p.group, max_chunks));
+    e = cudaMemsetAsync(p.counters, 0, (size_t)pairs * 4, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_error(e, name);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a->num_seqs, (unsigned)a->n_kv_heads, (unsigned)p.max_splits);
   cfg.blockDim = dim3(32u * warps, 1, 1);

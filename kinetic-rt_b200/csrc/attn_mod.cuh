@@ -9,7 +9,18 @@
 #include <cmath>
 #include <cstdint>
 
+#include "qkv_paged.cuh"
+
 namespace krt {
+
+// Workspaces of both attentions: status word and prompt queue in the header,
+// then decode's counters, then partial results.  What must be zero between
+// calls (queue, counters) lies at the same place for every call, of either
+// kind and of any size, and partial results never reach it: one buffer serves
+// all calls that follow one another.
+constexpr int kModCounters = 16384;  // (sequence, KV head) pairs; calls of more zero their own
+constexpr size_t kModCountersAt = kWsHeaderBytes;
+constexpr size_t kModPartsAt = kModCountersAt + kModCounters * 4;
 
 struct ScoreMod {
   float mul;         // scale * log2(e)

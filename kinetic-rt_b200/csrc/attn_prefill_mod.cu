@@ -1029,7 +1029,7 @@ extern "C" size_t krt_paged_attention_prefill_mod_workspace_size(int32_t num_tok
   const long long items = apm_items(num_tokens, num_seqs, n_heads, n_kv_heads);
   const long long worth = apm_worth(apm_blocks(max_kv_len));
   const size_t pieces = worth > 1 ? (size_t)std::min<long long>(apm_max_pieces(), items * worth) : 0;
-  return kWsHeaderBytes + pieces * (kApmPartBytes + kApmStatBytes);
+  return kModPartsAt + pieces * (kApmPartBytes + kApmStatBytes);
 }
 
 extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention_mod_args* a, void* stream) {
@@ -1112,8 +1112,8 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   p.items = (int)items;
   p.splits = (int)std::max(1ll, splits);
   p.piece = (int)piece;  // at least; `splits` of the item's real length otherwise
-  p.part_ml = reinterpret_cast<float2*>(ws + kWsHeaderBytes);
-  p.part_o = reinterpret_cast<float4*>(ws + kWsHeaderBytes + (size_t)items * p.splits * kApmStatBytes);
+  p.part_ml = reinterpret_cast<float2*>(ws + kModPartsAt);
+  p.part_o = reinterpret_cast<float4*>(ws + kModPartsAt + (size_t)items * p.splits * kApmStatBytes);
   CUtensorMap tmap_q, tmap_kv;
   int rc = make_tmap_bf16_5d_strided(&tmap_q, a->q, {64, (uint64_t)a->n_heads, (uint64_t)a->num_tokens, 2},
                                      {256, (uint64_t)a->q_stride * 2, 128},
