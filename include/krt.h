@@ -384,7 +384,8 @@ KRT_API int krt_paged_attention_prefill(const krt_paged_prefill_attention_args* 
  * may overlap on the GPU need workspaces of their own.  A workspace that is
  * large enough for each of them serves calls of both attentions, of any sizes,
  * heads and windows, one after another, captured ones too (other calls of this
- * header lay theirs out differently: not those).
+ * header lay theirs out differently: not those).  The size functions give 0 for
+ * shapes that the calls refuse.
  * ---------------------------------------------------------------------- */
 
 /* One query token per sequence, at position p = seq_lens[s] - 1 (its K/V are

@@ -525,7 +525,8 @@ size_t adm_part_bytes(long long pairs, int group, int max_chunks) {
 
 extern "C" size_t krt_paged_attention_mod_workspace_size(int32_t num_seqs, int32_t n_heads, int32_t n_kv_heads,
                                                          int32_t max_seq_len, int32_t window) {
-  if (num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || max_seq_len <= 0 || window < 0 || n_heads % n_kv_heads != 0)
+  if (num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || max_seq_len <= 0 || window < 0 ||
+      n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > kAdmMaxGroup)
     return 0;
   const long long pairs = (long long)num_seqs * n_kv_heads;
   const size_t own = pairs > kModCounters ? (size_t)pairs * 4 : 0;

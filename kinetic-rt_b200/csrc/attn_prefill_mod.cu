@@ -86,6 +86,7 @@ constexpr int kApmBlock = 64;    // keys per block
 constexpr int kApmPage = 16;     // tokens per TMA box
 constexpr int kApmStages = 4;    // of K, and of V
 constexpr int kApmSoftmaxWarps = 8;
+constexpr int kApmMaxGroup = 16;  // query heads per KV head
 constexpr int kApmThreads = 384;
 constexpr uint32_t kApmTileBytes = 32768;  // Q tile: 128 rows x 128 dims bf16, two [128 x 128 B] halves
 constexpr uint32_t kApmHalf = 16384;
@@ -1022,13 +1023,14 @@ long long apm_blocks(long long keys) { return (keys + kApmBlock - 1) / kApmBlock
 // ------------------------------------------------------------------ C ABI
 extern "C" size_t krt_paged_attention_prefill_mod_workspace_size(int32_t num_tokens, int32_t num_seqs, int32_t n_heads,
                                                                  int32_t n_kv_heads, int32_t max_kv_len) {
-  if (num_tokens <= 0 || num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 ||
-      max_kv_len <= 0)
+  if (num_tokens <= 0 || num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || max_kv_len <= 0 ||
+      n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > kApmMaxGroup)
     return 0;
   // status word, queue and flags; parts of items that are split
   const long long items = apm_items(num_tokens, num_seqs, n_heads, n_kv_heads);
   const long long worth = apm_worth(apm_blocks(max_kv_len));
-  const size_t pieces = worth > 1 ? (size_t)std::min<long long>(apm_max_pieces(), items * worth) : 0;
+  const long long most = apm_max_pieces();
+  const size_t pieces = worth > 1 ? (size_t)std::min(most, std::min(items, most) * worth) : 0;
   return kModPartsAt + pieces * (kApmPartBytes + kApmStatBytes);
 }
 
@@ -1040,7 +1042,7 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   if (a->head_dim != kHeadDim) return set_error(KRT_ERR_UNSUPPORTED, "%s: head_dim must be 128", name);
   if (a->num_tokens <= 0 || a->num_seqs <= 0 || a->n_heads <= 0 || a->n_kv_heads <= 0 || a->max_kv_len <= 0)
     return set_error(KRT_ERR_INVALID, "%s: num_tokens, num_seqs, heads and max_kv_len must be positive", name);
-  if (a->n_heads % a->n_kv_heads != 0 || a->n_heads / a->n_kv_heads > 16)
+  if (a->n_heads % a->n_kv_heads != 0 || a->n_heads / a->n_kv_heads > kApmMaxGroup)
     return set_error(KRT_ERR_UNSUPPORTED, "%s: n_heads must be a multiple of n_kv_heads, at most 16 per KV head", name);
   if (a->tokens_per_block <= 0 || a->tokens_per_block % kApmPage != 0)
     return set_error(KRT_ERR_UNSUPPORTED, "%s: tokens_per_block must be a multiple of 16", name);

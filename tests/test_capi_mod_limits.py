@@ -1,0 +1,29 @@
+"""Limits of the attention calls with score modifications, on the CPU: what the
+size functions answer for shapes that the calls refuse, and for the largest."""
+import os
+
+import pytest
+
+from python.kinetic_rt import _lib
+from tests.test_capi_mod_validation import FAKE, call, decode, prefill
+
+pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libkrt.so not built")
+
+BIG = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("group", [17, 32, 128, 129, 256, 4096])
+def test_no_workspace_for_groups_that_are_refused(group):
+    """More query heads per KV head than the kernels take: 0, as for other shapes that a call refuses."""
+    assert _lib.prefill_attention_mod_workspace_bytes(64, 1, group, 1, 4096) == 0
+    assert _lib.attention_mod_workspace_bytes(4, group, 1, 4096) == 0
+    assert _lib.prefill_attention_mod_workspace_bytes(64, 1, 16, 1, 4096) > 0
+    assert _lib.attention_mod_workspace_bytes(4, 16, 1, 4096) > 0
+
+
+def test_sizes_of_the_largest_shapes():
+    """No overflow: sizes grow with every argument up to its end."""
+    few = _lib.prefill_attention_mod_workspace_bytes(1, 1, 1, 1, BIG)
+    for args in ((BIG, 1, 1, 1, BIG), (BIG, BIG, 16, 1, BIG), (BIG, BIG, 16 * 65535, 65535, BIG)):
+        assert few <= _lib.prefill_attention_mod_workspace_bytes(*args) < 1 << 28
+    assert _lib.attention_mod_workspace_bytes(BIG, 16, 1, BIG) > _lib.attention_mod_workspace_bytes(1 << 20, 16, 1, BIG)
