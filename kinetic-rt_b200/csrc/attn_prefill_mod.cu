@@ -1042,7 +1042,7 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   if (a->head_dim != kHeadDim) return set_error(KRT_ERR_UNSUPPORTED, "%s: head_dim must be 128", name);
   if (a->num_tokens <= 0 || a->num_seqs <= 0 || a->n_heads <= 0 || a->n_kv_heads <= 0 || a->max_kv_len <= 0)
     return set_error(KRT_ERR_INVALID, "%s: num_tokens, num_seqs, heads and max_kv_len must be positive", name);
-  if (a->n_heads % a->n_kv_heads != 0 || a->n_heads / a->n_kv_heads > kApmMaxGroup)
+  if (a->n_heads % a->n_kv_heads != 0 || a->n_heads / a->n_kv_heads > kApmMaxGroup || a->n_kv_heads > 65535)
     return set_error(KRT_ERR_UNSUPPORTED, "%s: n_heads must be a multiple of n_kv_heads, at most 16 per KV head", name);
   if (a->tokens_per_block <= 0 || a->tokens_per_block % kApmPage != 0)
     return set_error(KRT_ERR_UNSUPPORTED, "%s: tokens_per_block must be a multiple of 16", name);

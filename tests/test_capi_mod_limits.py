@@ -27,3 +27,11 @@ def test_sizes_of_the_largest_shapes():
     for args in ((BIG, 1, 1, 1, BIG), (BIG, BIG, 16, 1, BIG), (BIG, BIG, 16 * 65535, 65535, BIG)):
         assert few <= _lib.prefill_attention_mod_workspace_bytes(*args) < 1 << 28
     assert _lib.attention_mod_workspace_bytes(BIG, 16, 1, BIG) > _lib.attention_mod_workspace_bytes(1 << 20, 16, 1, BIG)
+
+
+@pytest.mark.parametrize("fn,args", [("krt_paged_attention_decode_mod", decode), ("krt_paged_attention_prefill_mod", prefill)])
+@pytest.mark.parametrize("heads", [1 << 25, 16 * 65536])
+def test_more_heads_than_a_stride_can_tell(fn, args, heads):
+    """n_heads * 128 beyond 32 bits would let any row stride pass."""
+    rc, msg = call(fn, args(n_heads=heads, n_kv_heads=heads // 16, lse=FAKE, lse_stride=heads))
+    assert rc == _lib.KRT_ERR_UNSUPPORTED and "n_kv_heads" in msg, (rc, msg)
