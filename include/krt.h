@@ -422,7 +422,8 @@ KRT_API int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args* a
  * and out beyond q_start[num_seqs] are left as they were.  q_start must not
  * decrease nor leave 0 .. num_tokens (status bit 8; such parts are left out).
  * max_kv_len is an upper bound of len_s; a longer sequence is computed all
- * the same, within its block table (status bit 8 beyond it).  The workspace
+ * the same; keys beyond its row of the block table are not visible (status bit
+ * 8).  The workspace
  * holds partial sums of prompts whose keys are split over the GPU (60 MB at
  * most). */
 typedef struct krt_paged_prefill_attention_mod_args {

@@ -119,6 +119,7 @@ struct ApmParams {
   float2* part_ml;           // [piece][tile][row] reference and sum
   int32_t* part_flags;       // [piece][tile] V values that are not finite were taken out
   int num_tokens, num_seqs, bt_stride, num_blocks, tokens_per_block;
+  int key_end;  // positions that a row of the block table holds: no key beyond them is visited
   int n_kv_heads, group, tile_tokens;  // tile_tokens = 128 / group
   uint32_t group_inv;                  // row / group = row * group_inv >> 16 for rows below 128
   int out_stride, lse_stride;
@@ -185,6 +186,11 @@ __device__ __forceinline__ int apm_lowest(const ApmParams& p, int pos) {
   return p.mod.window > 0 ? max(0, pos - p.mod.window + 1) : 0;
 }
 
+// End of the keys that the query at `pos` of a sequence of `len` tokens sees.
+__device__ __forceinline__ int apm_highest(const ApmParams& p, int len, int prefix, int pos) {
+  return min(min(len, p.key_end), max(pos + 1, prefix));
+}
+
 // Item number `index` (seq -1: there are fewer, or q_start decreases somewhere
 // and they are more than num_tokens rows can give): sequences in order, the last
 // (heaviest) tokens of each first, KV heads innermost.  By a whole warp, 128
@@ -243,19 +249,23 @@ __device__ __forceinline__ ApmItem apm_find(const ApmParams& p, int index, int l
   it.lo_max = 0;
   it.hi_min = INT_MAX;
   const bool pos_ok = pos0 >= 0 && pos0 <= kApmMaxPos && q_len <= kApmMaxPos;
-  if (!pos_ok && lane == 0) atomicOr(p.status, kStatusBadBlock);
+  if ((!pos_ok || pos0 + q_len > p.key_end) && lane == 0) atomicOr(p.status, kStatusBadBlock);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     int lo_min = INT_MAX, hi_max = 0;  // over the tile's live rows
     const int from = tok0 + i * tt, to = min(from + tt, q_len) - 1;  // its tokens
     if (seq >= 0 && pos_ok && from <= to) {
-      auto highest = [&](int pos) { return min(pos0 + q_len, max(pos + 1, it.prefix)); };
+      auto highest = [&](int pos) { return apm_highest(p, pos0 + q_len, it.prefix, pos); };
       if (p.kv_start == nullptr) {
-        // every row is live; bounds do not decrease from token to token
-        lo_min = apm_lowest(p, pos0 + from);
-        hi_max = highest(pos0 + to);
-        it.lo_max = max(it.lo_max, apm_lowest(p, pos0 + to));
-        it.hi_min = min(it.hi_min, highest(pos0 + from));
+        // bounds do not decrease from token to token; every row is live but for
+        // those whose window lies beyond the block table
+        const int lo = apm_lowest(p, pos0 + from), hi = highest(pos0 + to);
+        if (lo < hi) {
+          lo_min = lo;
+          hi_max = hi;
+          it.lo_max = max(it.lo_max, apm_lowest(p, pos0 + to));
+          it.hi_min = min(it.hi_min, highest(pos0 + from));
+        }
       } else {
         int lo_max = 0, hi_min = INT_MAX;
         for (int tok = from + lane; tok <= to; tok += 32) {
@@ -644,7 +654,7 @@ __global__ void __launch_bounds__(kApmThreads, 1)
       const bool valid = r < tt * G && tok < at->q_len;
       if (valid && n > 0) {
         const int l = max(apm_lowest(p, pos), p.kv_start ? p.kv_start[at->t_first + tok] : 0);
-        const int h = min(at->pos0 + at->q_len, max(pos + 1, at->prefix));
+        const int h = apm_highest(p, at->pos0 + at->q_len, at->prefix, pos);
         live = l < h;
         if (live) {
           lo = l;
@@ -985,7 +995,7 @@ __global__ void __launch_bounds__(256) paged_attention_prefill_mod_join_kernel(c
   dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
   if (poison) {
     const int lo = max(apm_lowest(p, pos), p.kv_start ? p.kv_start[t] : 0);
-    apm_add_back(p, &it, lo, min(it.pos0 + it.q_len, max(pos + 1, it.prefix)), out, 16 * warp, 16 * warp + 16);
+    apm_add_back(p, &it, lo, apm_highest(p, it.pos0 + it.q_len, it.prefix, pos), out, 16 * warp, 16 * warp + 16);
   }
   if (p.lse && warp == 0)
     p.lse[(size_t)t * p.lse_stride + head] = L == 0.f ? -INFINITY : (M == -INFINITY ? L : (M + log2f(L)) * kLn2);
@@ -1086,6 +1096,7 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   p.bt_stride = a->block_table_stride;
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
+  p.key_end = (int)std::min<long long>((long long)a->block_table_stride * a->tokens_per_block, INT_MAX - kApmBlock);
   p.n_kv_heads = a->n_kv_heads;
   p.group = a->n_heads / a->n_kv_heads;
   p.tile_tokens = kApmRows / p.group;
