@@ -407,6 +407,7 @@ typedef struct krt_paged_attention_mod_args {
   float scale, softcap;
   void* workspace;
   size_t workspace_bytes;
+  int32_t block_table_columns; /* of a row; 0: block_table_stride. Columns beyond it are not read */
 } krt_paged_attention_mod_args;
 
 KRT_API size_t krt_paged_attention_mod_workspace_size(int32_t num_seqs, int32_t n_heads, int32_t n_kv_heads,
@@ -444,6 +445,7 @@ typedef struct krt_paged_prefill_attention_mod_args {
   float scale, softcap;
   void* workspace;
   size_t workspace_bytes;
+  int32_t block_table_columns; /* of a row; 0: block_table_stride. Columns beyond it are not read */
 } krt_paged_prefill_attention_mod_args;
 
 KRT_API size_t krt_paged_attention_prefill_mod_workspace_size(int32_t num_tokens, int32_t num_seqs, int32_t n_heads,
@@ -485,6 +487,7 @@ typedef struct krt_rope_append_args {
   float factor; /* on cos and sin; 0 = 1 */
   void* workspace; /* krt_rope_append_workspace_size() bytes, zeroed once: the status word */
   size_t workspace_bytes;
+  int32_t block_table_columns; /* of a row; 0: block_table_stride. Columns beyond it are not read */
 } krt_rope_append_args;
 
 KRT_API size_t krt_rope_append_workspace_size(void);

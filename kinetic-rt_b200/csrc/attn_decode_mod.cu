@@ -60,7 +60,7 @@ struct AdmParams {
   float* part;               // [num_seqs][n_kv_heads][max_splits][group][kAdmRowFloats]
   uint32_t* counters;        // [num_seqs][n_kv_heads], zero between calls
   int* status;
-  int bt_stride, num_blocks, tokens_per_block;
+  int bt_stride, bt_columns, num_blocks, tokens_per_block;
   int n_kv_heads, group;
   int q_stride, out_stride, lse_stride;
   int chunks_per_split, max_splits;
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
     const int tok = (c_begin + i) * kAdmChunk;
     const int col = tok / p.tokens_per_block;
     int v = -1;
-    if (col < p.bt_stride) {
+    if (col < p.bt_columns) {
       const int blk = p.block_table[(size_t)b * p.bt_stride + col];
       if (blk >= 0 && blk < p.num_blocks) v = blk * p.tokens_per_block + tok % p.tokens_per_block;
     }
@@ -547,9 +547,12 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
     return set_error(KRT_ERR_UNSUPPORTED, "%s: tokens_per_block must be a multiple of 16", name);
   if (a->num_blocks <= 0 || a->block_table_stride <= 0)
     return set_error(KRT_ERR_INVALID, "%s: paged-cache geometry must be positive", name);
+  const int columns = block_table_columns(a->block_table_columns, a->block_table_stride, a->num_seqs);
+  if (columns < 0)
+    return set_error(KRT_ERR_INVALID, "%s: block_table_columns must lie in 0 .. block_table_stride", name);
   if ((long long)a->num_blocks * a->tokens_per_block > INT_MAX - kAdmChunk)
     return set_error(KRT_ERR_UNSUPPORTED, "%s: the pool may hold fewer than 2^31 - 16 tokens", name);
-  if ((long long)a->block_table_stride * a->tokens_per_block < a->max_seq_len)
+  if ((long long)columns * a->tokens_per_block < a->max_seq_len)
     return set_error(KRT_ERR_INVALID, "%s: the block table cannot hold max_seq_len tokens", name);
   if (a->q_stride < a->n_heads * kHeadDim || a->q_stride % 8 != 0 || a->out_stride < a->n_heads * kHeadDim ||
       a->out_stride % 8 != 0)
@@ -580,6 +583,7 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   p.part = reinterpret_cast<float*>(ws + kModPartsAt);
   p.counters = reinterpret_cast<uint32_t*>(ws + kModCountersAt);
   p.bt_stride = a->block_table_stride;
+  p.bt_columns = columns;
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
   p.n_kv_heads = a->n_kv_heads;

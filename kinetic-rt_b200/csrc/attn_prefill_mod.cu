@@ -118,7 +118,7 @@ struct ApmParams {
   float4* part_o;            // [piece][tile][column / 4][row]
   float2* part_ml;           // [piece][tile][row] reference and sum
   int32_t* part_flags;       // [piece][tile] V values that are not finite were taken out
-  int num_tokens, num_seqs, bt_stride, num_blocks, tokens_per_block;
+  int num_tokens, num_seqs, bt_stride, bt_columns, num_blocks, tokens_per_block;
   int key_end;  // positions that a row of the block table holds: no key beyond them is visited
   int n_kv_heads, group, tile_tokens;  // tile_tokens = 128 / group
   uint32_t group_inv;                  // row / group = row * group_inv >> 16 for rows below 128
@@ -175,7 +175,7 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t w) { return ((w & 0x7F8
 // Pool slot of position j of the sequence, or -1.
 __device__ __forceinline__ long long apm_slot(const ApmParams& p, const int32_t* table, int j) {
   const int col = j / p.tokens_per_block;
-  if (col >= p.bt_stride) return -1;
+  if (col >= p.bt_columns) return -1;
   const int blk = table[col];
   if (blk < 0 || blk >= p.num_blocks) return -1;
   return (long long)blk * p.tokens_per_block + j % p.tokens_per_block;
@@ -1058,9 +1058,12 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
     return set_error(KRT_ERR_UNSUPPORTED, "%s: tokens_per_block must be a multiple of 16", name);
   if (a->num_blocks <= 0 || a->block_table_stride <= 0)
     return set_error(KRT_ERR_INVALID, "%s: paged-cache geometry must be positive", name);
+  const int columns = block_table_columns(a->block_table_columns, a->block_table_stride, a->num_seqs);
+  if (columns < 0)
+    return set_error(KRT_ERR_INVALID, "%s: block_table_columns must lie in 0 .. block_table_stride", name);
   if ((long long)a->num_blocks * a->tokens_per_block > INT_MAX - kApmPage)
     return set_error(KRT_ERR_UNSUPPORTED, "%s: the pool may hold fewer than 2^31 - 16 tokens", name);
-  if ((long long)a->block_table_stride * a->tokens_per_block < a->max_kv_len)
+  if ((long long)columns * a->tokens_per_block < a->max_kv_len)
     return set_error(KRT_ERR_INVALID, "%s: the block table cannot hold max_kv_len tokens", name);
   if (a->q_stride < a->n_heads * kHeadDim || a->q_stride % 8 != 0 || a->out_stride < a->n_heads * kHeadDim ||
       a->out_stride % 8 != 0)
@@ -1094,9 +1097,10 @@ extern "C" int krt_paged_attention_prefill_mod(const krt_paged_prefill_attention
   p.num_tokens = a->num_tokens;
   p.num_seqs = a->num_seqs;
   p.bt_stride = a->block_table_stride;
+  p.bt_columns = columns;
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
-  p.key_end = (int)std::min<long long>((long long)a->block_table_stride * a->tokens_per_block, INT_MAX - kApmBlock);
+  p.key_end = (int)std::min<long long>((long long)columns * a->tokens_per_block, INT_MAX - kApmBlock);
   p.n_kv_heads = a->n_kv_heads;
   p.group = a->n_heads / a->n_kv_heads;
   p.tile_tokens = kApmRows / p.group;

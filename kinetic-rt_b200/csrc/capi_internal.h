@@ -28,6 +28,13 @@ int make_tmap_pool_kv16(CUtensorMap* map, const void* pool, int num_blocks, int 
 int make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems,
                       uint32_t box_rows);
 
+// Columns of a block table row that may be read (0: as many as its stride), -1
+// where they are no part of it.
+inline int block_table_columns(int columns, int stride, int rows) {
+  if (columns < 0 || (columns > stride && rows > 1)) return -1;
+  return columns ? columns : stride;
+}
+
 // capi.cu: argument checks of krt_qkv_rope_decode, workspace excluded
 int decode_args_check(const krt_qkv_paged_args* a, const char* name);
 

@@ -53,7 +53,7 @@ struct RaParams {
   int* status;
   long long q_stride, k_stride, v_stride, q_out_stride;
   int num_tokens, n_heads, n_kv_heads, rotary_dim, interleaved;
-  int num_seqs, bt_stride, num_blocks, tokens_per_block;
+  int num_seqs, bt_stride, bt_columns, num_blocks, tokens_per_block;
   float factor;
 };
 
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kRaThreads, 4) rope_append_kernel(const RaPara
   long long slot = -1;  // in the pool; -1: k and v are not written
   const int at = p.cache_index ? p.cache_index[t] : position;
   const int col = at >= 0 ? at / p.tokens_per_block : -1;
-  if (seq < p.num_seqs && col >= 0 && col < p.bt_stride) {
+  if (seq < p.num_seqs && col >= 0 && col < p.bt_columns) {
     const int blk = p.block_table[(size_t)seq * p.bt_stride + col];
     if (blk >= 0 && blk < p.num_blocks)
       slot = (long long)blk * p.tokens_per_block + (at - col * p.tokens_per_block);
@@ -283,6 +283,9 @@ extern "C" int krt_rope_append(const krt_rope_append_args* a, void* stream) {
     return set_error(KRT_ERR_INVALID, "%s: tensors must be 16-byte aligned (inv_freq 8)", name);
   if (a->num_seqs <= 0 || a->block_table_stride <= 0 || a->num_blocks <= 0 || a->tokens_per_block <= 0)
     return set_error(KRT_ERR_INVALID, "%s: paged-cache geometry must be positive", name);
+  const int columns = block_table_columns(a->block_table_columns, a->block_table_stride, a->num_seqs);
+  if (columns < 0)
+    return set_error(KRT_ERR_INVALID, "%s: block_table_columns must lie in 0 .. block_table_stride", name);
   if (!std::isfinite(a->factor)) return set_error(KRT_ERR_INVALID, "%s: factor must be finite", name);
   if (a->workspace_bytes < kWsHeaderBytes)
     return set_error(KRT_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, a->workspace_bytes,
@@ -322,6 +325,7 @@ extern "C" int krt_rope_append(const krt_rope_append_args* a, void* stream) {
   p.interleaved = a->interleaved != 0;
   p.num_seqs = a->num_seqs;
   p.bt_stride = a->block_table_stride;
+  p.bt_columns = columns;
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
   p.factor = a->factor == 0.f ? 1.f : a->factor;

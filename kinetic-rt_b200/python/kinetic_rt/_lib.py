@@ -98,6 +98,7 @@ class PagedAttentionModArgs(ctypes.Structure):
         ("block_table_stride", _i32), ("num_blocks", _i32), ("tokens_per_block", _i32),
         ("max_seq_len", _i32), ("window", _i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
         ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("block_table_columns", _i32),
     ]
 
 
@@ -111,6 +112,7 @@ class PagedPrefillAttentionModArgs(ctypes.Structure):
         ("block_table_stride", _i32), ("num_blocks", _i32), ("tokens_per_block", _i32),
         ("max_kv_len", _i32), ("window", _i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
         ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("block_table_columns", _i32),
     ]
 
 
@@ -124,6 +126,7 @@ class RopeAppendArgs(ctypes.Structure):
         ("interleaved", _i32), ("dtype", _i32),
         ("num_seqs", _i32), ("block_table_stride", _i32), ("num_blocks", _i32), ("tokens_per_block", _i32),
         ("factor", ctypes.c_float), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("block_table_columns", _i32),
     ]
 
 
@@ -464,7 +467,7 @@ def _check_shape(who, name, t, *shape):
 def _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_heads):
     import torch
     _check_cuda(who, torch.int32, block_table=block_table)
-    if block_table.dim() != 2:
+    if block_table.dim() != 2 or block_table.shape[1] == 0:
         raise ValueError(f"{who}: block_table must be [num_seqs, blocks]")
     _check_cuda(who, torch.bfloat16, kv_pool=kv_pool)
     if not kv_pool.is_contiguous() or kv_pool.numel() < num_blocks * tokens_per_block * 2 * n_kv_heads * 128:
@@ -538,6 +541,7 @@ def attention_mod_args(q, kv_pool, block_table, seq_lens, out, n_heads, n_kv_hea
     a.scale, a.softcap = float(scale), float(softcap)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()
+    a.block_table_columns = int(block_table.shape[1])
     return _keep(a, device, q, kv_pool, block_table, seq_lens, out, lse, alibi_slopes, kv_start, workspace)
 
 
@@ -587,6 +591,7 @@ def prefill_attention_mod_args(q, kv_pool, block_table, q_start, q_pos0, out, n_
     a.scale, a.softcap = float(scale), float(softcap)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()
+    a.block_table_columns = int(block_table.shape[1])
     return _keep(a, device, q, kv_pool, block_table, q_start, q_pos0, out, lse, alibi_slopes, kv_start, prefix_lens,
                  workspace)
 
@@ -638,6 +643,7 @@ def rope_append_args(q, k, v, inv_freq, positions, token_seq, block_table, kv_po
     a.num_blocks, a.tokens_per_block, a.factor = int(num_blocks), int(tokens_per_block), float(factor)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()
+    a.block_table_columns = int(block_table.shape[1])
     return _keep(a, device, q, k, v, inv_freq, positions, cache_index, token_seq, block_table, kv_pool, q_out,
                  workspace)
 

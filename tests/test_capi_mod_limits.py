@@ -5,7 +5,7 @@ import os
 import pytest
 
 from python.kinetic_rt import _lib
-from tests.test_capi_mod_validation import FAKE, call, decode, prefill
+from tests.test_capi_mod_validation import FAKE, call, decode, prefill, rope
 
 pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libkrt.so not built")
 
@@ -35,3 +35,18 @@ def test_more_heads_than_a_stride_can_tell(fn, args, heads):
     """n_heads * 128 beyond 32 bits would let any row stride pass."""
     rc, msg = call(fn, args(n_heads=heads, n_kv_heads=heads // 16, lse=FAKE, lse_stride=heads))
     assert rc == _lib.KRT_ERR_UNSUPPORTED and "n_kv_heads" in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("over,text", [(dict(block_table_columns=62), "cannot hold"), (dict(block_table_columns=-1), "columns"),
+                                       (dict(block_table_columns=65), "columns")])
+@pytest.mark.parametrize("fn,args", [("krt_paged_attention_decode_mod", decode), ("krt_paged_attention_prefill_mod", prefill)])
+def test_block_table_columns(fn, args, over, text):
+    """The columns of a row, not its stride, have to hold the longest sequence (1000 tokens take 63 blocks of 16)."""
+    rc, msg = call(fn, args(**over))
+    assert rc == _lib.KRT_ERR_INVALID and text in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("columns", [-1, 5])
+def test_rope_append_block_table_columns(columns):
+    rc, msg = call("krt_rope_append", rope(block_table_columns=columns))
+    assert rc == _lib.KRT_ERR_INVALID and "columns" in msg, (rc, msg)

@@ -47,3 +47,68 @@ def test_prompt_beyond_its_table_with_prefix_and_starts(torch_cuda):  # noqa: F8
     c.launch(a)
     assert _lib.read_status(c.ws)[1] == 8
     hold(c, [(0, 2 ** 20 + i, 48, first[i], 10 ** 6) for i in range(40)])
+
+
+# ------------------------------------------------------------ column slices
+def sliced(torch, table, columns, last):
+    """The table as columns of a wider one whose other entries name no block (last: the slice ends with the memory)."""
+    S, n = table.shape
+    wide = torch.full((S, 3 * n), 2 ** 30, dtype=torch.int32, device="cuda")
+    at = 2 * n if last else n
+    wide[:, at:at + n] = torch.from_numpy(table).cuda()
+    return wide[:, at:at + columns]
+
+
+@pytest.mark.parametrize("last", [False, True])
+@pytest.mark.parametrize("q_lens", [None, [70, 30, 64]])
+def test_attention_on_a_slice_of_a_table(torch_cuda, q_lens, last):  # noqa: F811
+    torch = torch_cuda
+    c = Case(torch, [300, 17, 128], q_lens=q_lens, seed=92)
+    c.table_d = sliced(torch, c.table, c.table.shape[1], last)
+    c.check(softcap=30.0)
+
+
+@pytest.mark.parametrize("last", [False, True])
+def test_prompt_beyond_a_slice(torch_cuda, last):  # noqa: F811
+    """Keys end with the slice, though its row goes on."""
+    torch = torch_cuda
+    from python.kinetic_rt import _lib
+    c = Case(torch, [310, 100], q_lens=[74, 20], seed=93)
+    c.table_d = sliced(torch, c.table, 20, last)  # 320 of 384 positions
+    c.launch(c.args(max_len=320))
+    assert _lib.read_status(c.ws)[1] == 8
+    hold(c, [(0, 310 + i, 320, 0, 0) for i in range(74)] + [(1, 100 + i, 120, 0, 0) for i in range(20)])
+
+
+@pytest.mark.parametrize("q_lens", [None, [70, 30]])
+def test_bound_beyond_a_slice_is_refused(torch_cuda, q_lens):  # noqa: F811
+    torch = torch_cuda
+    c = Case(torch, [300, 100], q_lens=q_lens, seed=94)
+    c.table_d = sliced(torch, c.table, 10, False)
+    with pytest.raises(ValueError, match="cannot hold"):
+        c.launch(c.args())
+
+
+@pytest.mark.parametrize("last", [False, True])
+def test_append_to_a_slice(torch_cuda, last):  # noqa: F811
+    """Tokens within the slice go to their slots; one behind it is reported and left out, its q is rotated all the same."""
+    torch = torch_cuda
+    from python.kinetic_rt import _lib
+    H, K, tpb = 4, 2, 16
+    table = np.array([[3, 0, 5], [1, 4, 2]], np.int32)
+    x = torch.randn(4, (H + 2 * K) * 128, device="cuda").to(torch.bfloat16)
+    pool = torch.full((6, tpb, 2, K, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    q_out = torch.zeros(4, H * 128, dtype=torch.bfloat16, device="cuda")
+    ws = torch.zeros(_lib.rope_append_workspace_bytes(), dtype=torch.uint8, device="cuda")
+    index, seq = [0, 33, 47, 31], [0, 0, 1, 1]  # columns 0, 2 (beyond the slice), 2 (beyond), 1
+    f = 0.5 ** torch.arange(64, dtype=torch.float64, device="cuda")
+    cut = sliced(torch, table, 2, last)
+    _lib.rope_append(_lib.rope_append_args(x[:, :H * 128], x[:, H * 128:(H + K) * 128], x[:, (H + K) * 128:], f,
+                                           i32(torch, [0] * 4), i32(torch, seq), cut, pool, q_out, H, K, 6, tpb, ws,
+                                           cache_index=i32(torch, index)))
+    assert _lib.read_status(ws)[1] == 8
+    assert torch.equal(q_out, x[:, :H * 128])  # position 0: not turned
+    want = torch.full_like(pool, 7.0)
+    for t, (b, o) in ((0, (3, 0)), (3, (4, 15))):
+        want[b, o] = x[t, H * 128:].view(2, K, 128)
+    assert torch.equal(pool, want)
