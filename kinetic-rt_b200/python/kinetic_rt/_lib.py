@@ -464,6 +464,12 @@ def _check_shape(who, name, t, *shape):
         raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, at least {shape} is needed")
 
 
+def _row_stride(t, width):
+    """Elements from row to row; of a single row, which may come with any
+    stride, the `width` that is used of it."""
+    return int(t.stride(0)) if t.shape[0] > 1 else width
+
+
 def _check_cache(who, kv_pool, block_table, num_blocks, tokens_per_block, n_kv_heads):
     import torch
     _check_cuda(who, torch.int32, block_table=block_table)
@@ -534,9 +540,9 @@ def attention_mod_args(q, kv_pool, block_table, seq_lens, out, n_heads, n_kv_hea
                                                         _ptr(out))
     a.lse, a.alibi_slopes, a.kv_start = _ptr(lse), _ptr(alibi_slopes), _ptr(kv_start)
     a.num_seqs, a.n_heads, a.n_kv_heads, a.head_dim = S, H, int(n_kv_heads), int(head_dim)
-    a.q_stride, a.out_stride = int(q.stride(0)), int(out.stride(0))
-    a.lse_stride = 0 if lse is None else int(lse.stride(0))
-    a.block_table_stride, a.num_blocks = int(block_table.stride(0)), int(num_blocks)
+    a.q_stride, a.out_stride = _row_stride(q, H * head_dim), _row_stride(out, H * head_dim)
+    a.lse_stride = 0 if lse is None else _row_stride(lse, H)
+    a.block_table_stride, a.num_blocks = _row_stride(block_table, int(block_table.shape[1])), int(num_blocks)
     a.tokens_per_block, a.max_seq_len, a.window = int(tokens_per_block), int(max_seq_len), int(window)
     a.scale, a.softcap = float(scale), float(softcap)
     a.workspace = _ptr(workspace)
@@ -584,9 +590,9 @@ def prefill_attention_mod_args(q, kv_pool, block_table, q_start, q_pos0, out, n_
     a.q_start, a.q_pos0, a.lse, a.alibi_slopes = _ptr(q_start), _ptr(q_pos0), _ptr(lse), _ptr(alibi_slopes)
     a.kv_start, a.prefix_lens = _ptr(kv_start), _ptr(prefix_lens)
     a.num_tokens, a.num_seqs, a.n_heads, a.n_kv_heads, a.head_dim = T, S, H, int(n_kv_heads), int(head_dim)
-    a.q_stride, a.out_stride = int(q.stride(0)), int(out.stride(0))
-    a.lse_stride = 0 if lse is None else int(lse.stride(0))
-    a.block_table_stride, a.num_blocks = int(block_table.stride(0)), int(num_blocks)
+    a.q_stride, a.out_stride = _row_stride(q, H * head_dim), _row_stride(out, H * head_dim)
+    a.lse_stride = 0 if lse is None else _row_stride(lse, H)
+    a.block_table_stride, a.num_blocks = _row_stride(block_table, int(block_table.shape[1])), int(num_blocks)
     a.tokens_per_block, a.max_kv_len, a.window = int(tokens_per_block), int(max_kv_len), int(window)
     a.scale, a.softcap = float(scale), float(softcap)
     a.workspace = _ptr(workspace)
@@ -635,11 +641,12 @@ def rope_append_args(q, k, v, inv_freq, positions, token_seq, block_table, kv_po
     a.q, a.k, a.v, a.inv_freq, a.positions = _ptr(q), _ptr(k), _ptr(v), _ptr(inv_freq), _ptr(positions)
     a.cache_index, a.token_seq, a.block_table = _ptr(cache_index), _ptr(token_seq), _ptr(block_table)
     a.kv_pool, a.q_out = _ptr(kv_pool), _ptr(q_out)
-    a.q_stride, a.k_stride, a.v_stride = int(q.stride(0)), int(k.stride(0)), int(v.stride(0))
-    a.q_out_stride = int(q_out.stride(0))
+    a.q_stride, a.q_out_stride = _row_stride(q, H * head_dim), _row_stride(q_out, H * head_dim)
+    a.k_stride, a.v_stride = _row_stride(k, K * head_dim), _row_stride(v, K * head_dim)
     a.num_tokens, a.n_heads, a.n_kv_heads, a.head_dim = T, H, K, int(head_dim)
     a.rotary_dim, a.interleaved, a.dtype = 2 * int(inv_freq.shape[0]), int(bool(interleaved)), _dtype_code(q)
-    a.num_seqs, a.block_table_stride = int(block_table.shape[0]), int(block_table.stride(0))
+    a.num_seqs = int(block_table.shape[0])
+    a.block_table_stride = _row_stride(block_table, int(block_table.shape[1]))
     a.num_blocks, a.tokens_per_block, a.factor = int(num_blocks), int(tokens_per_block), float(factor)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = workspace.numel() * workspace.element_size()

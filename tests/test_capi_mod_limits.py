@@ -50,3 +50,10 @@ def test_block_table_columns(fn, args, over, text):
 def test_rope_append_block_table_columns(columns):
     rc, msg = call("krt_rope_append", rope(block_table_columns=columns))
     assert rc == _lib.KRT_ERR_INVALID and "columns" in msg, (rc, msg)
+
+
+def test_row_stride_of_one_row():
+    torch = pytest.importorskip("torch")
+    assert _lib._row_stride(torch.empty(512, 1).T, 512) == 512
+    assert _lib._row_stride(torch.empty(1, 520)[:, :512], 512) == 512
+    assert _lib._row_stride(torch.empty(2, 520)[:, :512], 512) == 520

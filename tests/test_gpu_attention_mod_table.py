@@ -112,3 +112,35 @@ def test_append_to_a_slice(torch_cuda, last):  # noqa: F811
     for t, (b, o) in ((0, (3, 0)), (3, (4, 15))):
         want[b, o] = x[t, H * 128:].view(2, K, 128)
     assert torch.equal(pool, want)
+
+
+# ------------------------------------------------------------- single rows
+def turned(t):
+    """A tensor of one row whose row stride is 1, as a transposed column has it."""
+    assert t.shape[0] == 1
+    u = t.reshape(-1, 1).clone().T
+    assert u.stride(0) == 1 and u.shape == t.shape
+    return u
+
+
+@pytest.mark.parametrize("q_lens", [None, [1]])
+def test_attention_of_one_row_of_any_stride(torch_cuda, q_lens):  # noqa: F811
+    torch = torch_cuda
+    c = Case(torch, [300], q_lens=q_lens, seed=95)
+    c.q_d, c.out, c.lse, c.table_d = (turned(t) for t in (c.q_d, c.out, c.lse, c.table_d))
+    c.check(softcap=30.0)
+
+
+def test_append_of_one_row_of_any_stride(torch_cuda):  # noqa: F811
+    torch = torch_cuda
+    from python.kinetic_rt import _lib
+    H, K = 4, 2
+    q, k, v = (turned(torch.randn(1, n * 128, device="cuda").to(torch.bfloat16)) for n in (H, K, K))
+    pool = torch.zeros(2, 16, 2, K, 128, dtype=torch.bfloat16, device="cuda")
+    q_out = turned(torch.zeros(1, H * 128, dtype=torch.bfloat16, device="cuda"))
+    ws = torch.zeros(_lib.rope_append_workspace_bytes(), dtype=torch.uint8, device="cuda")
+    f = 0.5 ** torch.arange(64, dtype=torch.float64, device="cuda")
+    _lib.rope_append(_lib.rope_append_args(q, k, v, f, i32(torch, [0]), i32(torch, [0]), turned(i32(torch, [[1, 0]])), pool,
+                                           q_out, H, K, 2, 16, ws, cache_index=i32(torch, [19])))
+    assert _lib.read_status(ws) == (0, 0)
+    assert torch.equal(q_out, q) and torch.equal(pool[0, 3, 0].reshape(1, -1), k) and torch.equal(pool[0, 3, 1].reshape(1, -1), v)
