@@ -56,16 +56,33 @@ def rope_cache(torch, max_position, head_dim, theta, device="cuda"):
     return emb.cos().float().to(device), emb.sin().float().to(device)
 
 
-def rope_inv_freq(torch, rotary_dim, theta, stretch=1.0, trained_context=8192, device="cuda"):
+def rope_inv_freq(torch, rotary_dim, theta, stretch=1.0, trained_context=8192, device="cuda", scaling="llama3"):
     """Rotary frequencies of rope_append (fp64 [rotary_dim / 2]) and the factor
-    on cos and sin that goes with them.  stretch > 1 scales for long contexts:
-    a frequency that makes fewer than one turn in `trained_context` tokens is
-    divided by `stretch`, one that makes more than four is kept, those between
-    are blended; the factor is 0.1 ln(stretch) + 1."""
+    on cos and sin that goes with them.  stretch > 1 scales for contexts of
+    stretch * trained_context tokens, in one of two published ways; both keep
+    high frequencies, divide low ones by `stretch` and blend those between:
+      "llama3"  by the turns that a frequency makes in the trained context: kept
+                from four on, divided up to one, linear between; factor 1 (the
+                long-context form of the Llama 3 family)
+      "yarn"    by the frequency's index: kept up to the last index of at least
+                32 turns, divided from the first of at most one, linear between;
+                factor 0.1 ln(stretch) + 1"""
     import math
+    if not stretch >= 1.0:
+        raise ValueError(f"rope_inv_freq: stretch must be at least 1, found {stretch}")
     f = float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
-    keep = ((trained_context * f / (2 * math.pi) - 1) / 3).clamp(0, 1)
-    return (f * keep + f / stretch * (1 - keep)).to(device), 0.1 * math.log(stretch) + 1
+    if scaling == "llama3":
+        keep, factor = ((trained_context * f / (2 * math.pi) - 1) / 3).clamp(0, 1), 1.0
+    elif scaling == "yarn":
+        def index_of(turns):
+            return rotary_dim * math.log(trained_context / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        first, last = max(math.floor(index_of(32)), 0), min(math.ceil(index_of(1)), rotary_dim - 1)
+        index = torch.arange(rotary_dim // 2, dtype=torch.float64)
+        keep = 1 - ((index - first) / max(last - first, 1e-3)).clamp(0, 1)
+        factor = 0.1 * math.log(stretch) + 1
+    else:
+        raise ValueError(f"rope_inv_freq: scaling must be 'llama3' or 'yarn', found {scaling!r}")
+    return (f * keep + f / stretch * (1 - keep)).to(device), factor
 
 
 def vocab_shard(vocab, rank, world):
