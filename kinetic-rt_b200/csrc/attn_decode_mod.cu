@@ -66,6 +66,7 @@ struct AdmParams {
   int chunks_per_split, max_splits;
   int cluster;               // the splits of a (sequence, KV head) are one cluster
   int max_len;
+  int wide_cap;              // small scores take the cap's polynomial
   ScoreMod mod;
 };
 
@@ -239,6 +240,7 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
       for (int e = 0; e < 4; ++e) {
         const int tk = 8 * j + 2 * t4 + (e & 1);
         float v = CAP ? cap_score(sc[j][e], p.mod.cap_in, p.mod.cap2) : sc[j][e] * p.mod.mul;
+        if (CAP && p.wide_cap && fabsf(sc[j][e]) <= p.mod.poly_max) v = cap_at(sc[j][e], p.mod.poly);
         if (BIAS) v = fmaf(-slope2[e >> 1], (float)(pos - tok_base - tk), v);  // j <= pos: the distance is >= 0
         if (tk < v0 || tk >= v1) v = -INFINITY;
         sc[j][e] = v;
@@ -612,6 +614,10 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   if (p.max_splits == 1 || (p.cluster && adm_clusters(cap, bias, p.max_splits) < pairs)) p.cluster = 0;
   if (p.max_splits > 65535) return set_error(KRT_ERR_UNSUPPORTED, "%s: max_seq_len is too long", name);
   p.mod = make_score_mod(a->scale, a->softcap, a->alibi_slopes, a->window);
+  // The cap's exponent form is off by 2e-7 of the cap, up to 100 less than 1 % of
+  // the weights' rounding to bf16; beyond, small scores take the polynomial too
+  // (always: 341 us for 128 sequences of 4224, never: 329).
+  p.wide_cap = a->softcap > 100.f;
   CUtensorMap tmap;
   int rc = make_tmap_pool_kv16(&tmap, a->kv_pool, a->num_blocks, a->tokens_per_block, a->n_kv_heads, true);
   if (rc) return rc;

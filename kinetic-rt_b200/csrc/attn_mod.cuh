@@ -6,6 +6,7 @@
 // and the key is visible iff lo <= j < hi.  The kernels keep x in base 2
 // (times log2 e), where the softmax needs one ex2 per score.
 #pragma once
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -38,22 +39,32 @@ inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, 
   ScoreMod m;
   const float sc = scale > 0.f ? scale : 0.08838834764831845f;  // 1 / sqrt(128)
   m.mul = sc * kLog2e;
-  m.cap2 = softcap * kLog2e;
-  m.cap_in = softcap > 0.f ? 2.f * kLog2e * sc / softcap : 0.f;
+  m.cap2 = (float)std::min((double)softcap * kLog2e, 1.5e38);
+  m.cap_in = softcap > 0.f ? std::min(2.f * kLog2e * sc / softcap, 1e38f) : 0.f;
   m.slopes = slopes;
   m.window = window;
-  // cap2 * tanh(u), u = a s, as an odd polynomial in s (cap_poly's coefficients times cap2 a^(2k+1));
-  // left out where powers of a could leave the range of a float
   m.poly_max = -1.f;
   for (int k = 0; k < 5; ++k) m.poly[k] = make_float2(0.f, 0.f);
   if (softcap > 0.f) {
-    static const double c[5] = {0.9999985098838806, -0.33326974511146545, 0.13257454335689545, -0.05019525811076164,
-                                0.013194185681641102};
+    // cap2 * tanh(u), u = a s, as an odd polynomial in s: coefficients of u^(2k+1)
+    // times cap2 a^(2k+1) (cap2 a = mul).  cap_poly's where their powers of a keep
+    // within the range of a float.  For a larger cap (a softcap of 884 at the usual
+    // scale) the scores that matter are small beside it: the series of tanh, whose
+    // next term is below 1e-8 of the first up to u_max.
+    static const double fit[5] = {0.9999985098838806, -0.33326974511146545, 0.13257454335689545, -0.05019525811076164,
+                                  0.013194185681641102};
+    static const double series[3] = {1.0, -1.0 / 3, 2.0 / 15};
     const double a = (double)sc / softcap;
-    if (a > 1e-4 && a < 1e3 && softcap < 1e6f) {
-      double f = a * m.cap2;
-      for (int k = 0; k < 5; ++k, f *= a * a) m.poly[k] = make_float2((float)(c[k] * f), (float)(c[k] * f));
-      m.poly_max = (float)(0.7 / a);
+    const bool fitted = a > 1e-4 && a < 1e3 && softcap < 1e6f;
+    const int terms = fitted ? 5 : a > 1e-9 ? 3 : a > 1e-18 ? 2 : 1;
+    const double u_max = fitted ? 0.7 : terms == 3 ? 0.05 : terms == 2 ? 1e-3 : 1e-4;
+    if (a < 1e3) {
+      double f = fitted ? a * m.cap2 : (double)m.mul;
+      for (int k = 0; k < terms; ++k, f *= a * a) {
+        const float c = (float)((fitted ? fit : series)[k] * f);
+        m.poly[k] = make_float2(c, c);
+      }
+      m.poly_max = (float)std::min(u_max / a, 1e18);  // its square is a float too
     }
   }
   return m;
