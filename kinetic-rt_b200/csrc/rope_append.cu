@@ -290,16 +290,21 @@ extern "C" int krt_rope_append(const krt_rope_append_args* a, void* stream) {
   if (a->workspace_bytes < kWsHeaderBytes)
     return set_error(KRT_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, a->workspace_bytes,
                      (size_t)kWsHeaderBytes);
-  // q_out may not lie over q, k or v: a pair's two halves can belong to different threads
-  const size_t in_size = dtype == KRT_DTYPE_FLOAT32 ? 4 : 2;
-  const uintptr_t o0 = reinterpret_cast<uintptr_t>(a->q_out);
-  const uintptr_t o1 = o0 + ((size_t)(a->num_tokens - 1) * a->q_out_stride + (size_t)a->n_heads * kHeadDim) * 2;
+  // q_out may not lie over q, k or v: a pair's two halves can belong to different
+  // threads.  Rows of one pitch may alternate (columns of one wider tensor).
+  const uint64_t in_size = dtype == KRT_DTYPE_FLOAT32 ? 4 : 2;
+  const uint64_t o0 = reinterpret_cast<uintptr_t>(a->q_out), o_row = (uint64_t)a->n_heads * kHeadDim * 2;
+  const uint64_t o_pitch = (uint64_t)a->q_out_stride * 2, o1 = o0 + (a->num_tokens - 1) * o_pitch + o_row;
   const struct { const void* p; int64_t stride; int heads; } ins[3] = {
       {a->q, a->q_stride, a->n_heads}, {a->k, a->k_stride, a->n_kv_heads}, {a->v, a->v_stride, a->n_kv_heads}};
   for (const auto& in : ins) {
-    const uintptr_t i0 = reinterpret_cast<uintptr_t>(in.p);
-    const uintptr_t i1 = i0 + ((size_t)(a->num_tokens - 1) * in.stride + (size_t)in.heads * kHeadDim) * in_size;
-    if (o0 < i1 && i0 < o1) return set_error(KRT_ERR_INVALID, "%s: q_out overlaps an input", name);
+    const uint64_t row = (uint64_t)in.heads * kHeadDim * in_size, pitch = (uint64_t)in.stride * in_size;
+    const uint64_t i0 = reinterpret_cast<uintptr_t>(in.p), i1 = i0 + (a->num_tokens - 1) * pitch + row;
+    if (o0 >= i1 || i0 >= o1) continue;
+    // bytes from the start of an input row to that of the first q_out row behind it
+    const uint64_t ahead = o0 >= i0 ? (o0 - i0) % pitch : (pitch - (i0 - o0) % pitch) % pitch;
+    if (pitch == o_pitch && ahead >= row && ahead + o_row <= pitch) continue;
+    return set_error(KRT_ERR_INVALID, "%s: q_out overlaps an input", name);
   }
   RaParams p;
   std::memset(&p, 0, sizeof(p));

@@ -57,3 +57,14 @@ def test_row_stride_of_one_row():
     assert _lib._row_stride(torch.empty(512, 1).T, 512) == 512
     assert _lib._row_stride(torch.empty(1, 520)[:, :512], 512) == 512
     assert _lib._row_stride(torch.empty(2, 520)[:, :512], 512) == 520
+
+
+@pytest.mark.parametrize("at", [0, 16, 2032, 2048, 2304, 2544, 6160, -16, 2064 + 5 * 8192])
+def test_rope_append_rows_that_share_columns(at):
+    """Ten rows of 8192 bytes with q in [0, 2048), k in [2048, 2304) and v in [2304, 2560).  q_out's rows (2048 bytes, of
+    the same pitch) overlap one of them unless they start in 2560 .. 6144."""
+    q = FAKE + (1 << 20)
+    over = dict(n_kv_heads=1, q=q, k=q + 2048, v=q + 2304, q_out=q + at, q_stride=4096, k_stride=4096, v_stride=4096,
+                q_out_stride=4096)
+    rc, msg = call("krt_rope_append", rope(**over))
+    assert rc == _lib.KRT_ERR_INVALID and "overlaps" in msg, (rc, msg)
