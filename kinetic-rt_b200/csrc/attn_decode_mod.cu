@@ -60,13 +60,12 @@ struct AdmParams {
   float* part;               // [num_seqs][n_kv_heads][max_splits][group][kAdmRowFloats]
   uint32_t* counters;        // [num_seqs][n_kv_heads], zero between calls
   int* status;
-  int bt_stride, bt_columns, num_blocks, tokens_per_block;
+  int bt_stride, num_blocks, tokens_per_block;
   int n_kv_heads, group;
   int q_stride, out_stride, lse_stride;
   int chunks_per_split, max_splits;
   int cluster;               // the splits of a (sequence, KV head) are one cluster
   int max_len;
-  int wide_cap;              // small scores take the cap's polynomial
   ScoreMod mod;
 };
 
@@ -132,16 +131,12 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
   const int c_begin = chunk0 + z * p.chunks_per_split;
   const int c_count = min(chunk0 + n_chunks, c_begin + p.chunks_per_split) - c_begin;
 
-  // First pool token of every chunk of this CTA (-1 when the block table
-  // column or the block id is out of range: the chunk is masked).
+  // First pool token of every chunk of this CTA (-1 when the block id is out of
+  // range: the chunk is masked).  The table holds the column: len <= max_len.
   for (int i = threadIdx.x; i < c_count; i += kAdmThreads) {
     const int tok = (c_begin + i) * kAdmChunk;
-    const int col = tok / p.tokens_per_block;
-    int v = -1;
-    if (col < p.bt_columns) {
-      const int blk = p.block_table[(size_t)b * p.bt_stride + col];
-      if (blk >= 0 && blk < p.num_blocks) v = blk * p.tokens_per_block + tok % p.tokens_per_block;
-    }
+    const int blk = p.block_table[(size_t)b * p.bt_stride + tok / p.tokens_per_block];
+    const int v = blk >= 0 && blk < p.num_blocks ? blk * p.tokens_per_block + tok % p.tokens_per_block : -1;
     if (v < 0) atomicOr(p.status, kStatusBadBlock);
     tl->tok[i] = v;
   }
@@ -240,7 +235,7 @@ __global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
       for (int e = 0; e < 4; ++e) {
         const int tk = 8 * j + 2 * t4 + (e & 1);
         float v = CAP ? cap_score(sc[j][e], p.mod.cap_in, p.mod.cap2) : sc[j][e] * p.mod.mul;
-        if (CAP && p.wide_cap && fabsf(sc[j][e]) <= p.mod.poly_max) v = cap_at(sc[j][e], p.mod.poly);
+        if (CAP && p.mod.wide_cap && fabsf(sc[j][e]) <= p.mod.poly_max) v = cap_at(sc[j][e], p.mod.poly);
         if (BIAS) v = fmaf(-slope2[e >> 1], (float)(pos - tok_base - tk), v);  // j <= pos: the distance is >= 0
         if (tk < v0 || tk >= v1) v = -INFINITY;
         sc[j][e] = v;
@@ -585,7 +580,6 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   p.part = reinterpret_cast<float*>(ws + kModPartsAt);
   p.counters = reinterpret_cast<uint32_t*>(ws + kModCountersAt);
   p.bt_stride = a->block_table_stride;
-  p.bt_columns = columns;
   p.num_blocks = a->num_blocks;
   p.tokens_per_block = a->tokens_per_block;
   p.n_kv_heads = a->n_kv_heads;
@@ -617,7 +611,7 @@ extern "C" int krt_paged_attention_decode_mod(const krt_paged_attention_mod_args
   // The cap's exponent form is off by 2e-7 of the cap, up to 100 less than 1 % of
   // the weights' rounding to bf16; beyond, small scores take the polynomial too
   // (always: 341 us for 128 sequences of 4224, never: 329).
-  p.wide_cap = a->softcap > 100.f;
+  p.mod.wide_cap = a->softcap > 100.f;
   CUtensorMap tmap;
   int rc = make_tmap_pool_kv16(&tmap, a->kv_pool, a->num_blocks, a->tokens_per_block, a->n_kv_heads, true);
   if (rc) return rc;

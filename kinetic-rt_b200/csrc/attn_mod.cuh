@@ -29,6 +29,7 @@ struct ScoreMod {
   float cap_in;      // 2 * log2(e) * scale / cap: ex2(s * cap_in) = e^(2 x / c)
   const float* slopes;  // [n_heads] or NULL
   int window;        // 0 = none
+  int wide_cap;      // decode: small scores take the cap's polynomial
   // cap by polynomial while |s| <= poly_max: x = s * P(s^2), see cap_poly
   float2 poly[5];    // each coefficient twice: operands of packed multiply-adds
   float poly_max;    // negative: never
@@ -43,6 +44,7 @@ inline ScoreMod make_score_mod(float scale, float softcap, const float* slopes, 
   m.cap_in = softcap > 0.f ? std::min(2.f * kLog2e * sc / softcap, 1e38f) : 0.f;
   m.slopes = slopes;
   m.window = window;
+  m.wide_cap = 0;
   m.poly_max = -1.f;
   for (int k = 0; k < 5; ++k) m.poly[k] = make_float2(0.f, 0.f);
   if (softcap > 0.f) {
