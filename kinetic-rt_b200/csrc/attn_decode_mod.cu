@@ -14,12 +14,14 @@
 // swizzled; 192 KB under way per SM); Q K^T and P V on mma.sync m16n8k16 with
 // the group's query heads in the rows (about 4 FLOP a byte: the tensor rate
 // does not matter), statistics and sums in fp32; P is rounded to bf16 for P V
-// (relative 2^-9, as V is).  Warps merge in shared memory; splits through the
-// shared memory of a cluster, or in the workspace by the last CTA to finish;
-// always in split order, so results do not depend on which CTA that is.
-// Measured: 128 sequences of 4224 tokens, 8 KV heads (2.2 GB) in 321 us =
-// 6.9 TB/s; one sequence of 4224 tokens 9.0 us in a graph, of which about 5 are
-// the launch, a CTA's start and its merges.
+// (relative 2^-8 at most, as V is).  Warps merge in shared memory; splits
+// through the shared memory of a cluster, or in the workspace by the last CTA to
+// finish; always in split order, so results do not depend on which CTA that is.
+// Measured: 128 sequences of 4224 tokens, 8 KV heads (2.2 GB) in 323 to 346 us
+// (on different GPUs) = 6.4 to 6.9 TB/s; one sequence of 4224 tokens 9.5 us in a
+// graph of such calls, of which about 5 are the launch, a CTA's start and its
+// merges.  Pieces follow max_seq_len, not the lengths: that sequence under a
+// bound of 32768 takes 17.7 us, of 131072 30.2.
 //
 // V rows of tokens that are not visible are set to zero in shared memory
 // before P V: their weight is 0, and 0 * inf or 0 * NaN from a cache slot

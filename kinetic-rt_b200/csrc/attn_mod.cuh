@@ -87,9 +87,9 @@ __device__ __forceinline__ float rcp_approx(float x) {
 
 // s -> cap2 * tanh(scale * s / c) = cap2 - 2 cap2 / (1 + e^(2 x / c)).  The
 // form saturates without overflow checks (ex2 = inf gives +cap, 0 gives -cap)
-// and is off by about 2e-7 * cap2 near zero (one rounding each of 1 + e and of
-// the difference), where the hardware tanh would be off by 5e-4 * cap2: more
-// than the bf16 rounding of the weights at a cap of 50.
+// and is off by about 2e-7 * cap2, also near zero (one rounding each of 1 + e
+// and of the difference), where the hardware tanh would be off by 5e-4 * cap2:
+// more than the bf16 rounding of the weights at a cap of 50.
 __device__ __forceinline__ float cap_score(float s, float cap_in, float cap2) {
   const float e = ex2(s * cap_in);
   return fmaf(-2.f * cap2, rcp_approx(1.f + e), cap2);
@@ -130,9 +130,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // P(w), w = s^2, of cap2 * tanh(scale s / c) = s * P(s^2) for |u| = |scale s /
 // c| <= 0.7: the degree-4 polynomial in u^2 with the smallest largest error of
 // u * P(u^2) against tanh(u) there (fitted by reweighted least squares), off
-// by at most 9.5e-8.  Scores beyond that take cap_score.  Five multiply-adds
-// and no special-function operation, of which the softmax needs all: tanh by
-// ex2 and rcp would triple them.
+// by at most 9.94e-8, and 1.5e-6 of tanh(u).  Scores beyond that take cap_score;
+// a cap outside the coefficients' range takes tanh's series (make_score_mod).
+// Five multiply-adds and no special-function operation, of which the softmax
+// needs all: tanh by ex2 and rcp would triple them.
 __device__ __forceinline__ f32x2 cap_poly(f32x2 w, const f32x2* c) {
   return fma2(fma2(fma2(fma2(c[4], w, c[3]), w, c[2]), w, c[1]), w, c[0]);
 }

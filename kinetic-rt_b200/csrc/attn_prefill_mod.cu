@@ -34,7 +34,7 @@
 // Few rows behind a long cache make fewer items than there are SMs; their keys
 // are then split into pieces (of eight blocks at least), whose unnormalised
 // sums a second kernel joins.  Measured, 8 tokens of 8 KV heads behind 65536:
-// 726 us whole, 64 split; behind 8192: 100 and 25; behind 1024: 19 and 17.
+// 726 us whole, 64 split; behind 8192: 100 and 25 to 28; behind 1024: 19 and 17.
 // (Pieces of four blocks: 14 there, but a 512-token prompt takes 20 for 17.)
 // The last items of a long causal prompt are split too where the others would
 // end well before them.
@@ -44,9 +44,10 @@
 // per 32 cycles of it), the special-function units 2048 for one ex2 a score.
 // A step takes about 3500 without and 4500 with a cap: the softmax warps' issue
 // slots (the cap's polynomial, maxima, packing) come on top of what the
-// special-function units leave of them.  Measured: six chunks of 517 tokens
-// behind 3700, 64 heads, 296 us = 957 TFLOP/s; 8 x 2048, 32 heads, causal,
-// capped, 357 us = 770 TFLOP/s; 64 tokens alone, 9.9 us in a graph.
+// special-function units leave of them.  Measured at full clock: six chunks of
+// 517 tokens behind 3700, 64 heads, 289 us = 982 TFLOP/s; 8 x 2048, 32 heads,
+// causal, capped, 355 us = 775 TFLOP/s; 64 tokens alone, 9.9 us in a graph.
+// Under the power cap of long runs 322 and 391 us.
 // Steps that are spared:
 //   * the reference that scores are taken against is the row's old maximum
 //     unless it grew by more than 2^16 (weights then stay below that, and bf16
@@ -58,8 +59,10 @@
 //   * the cap is a polynomial of the score while scores are well below it, and
 //     its value at the row's largest |score| serves as the reference.
 //
-// Statistics, sums and O are fp32; P is rounded to bf16 for P V (2^-9 of each
-// weight, as V is).
+// Statistics, sums and O are fp32; P is rounded to bf16 for P V (2^-8 of each
+// weight at most, as V is).  Beside the split of its keys, a row's bits depend on
+// its sequence alone: not on the next one's rows in its tile, unwritten cache
+// slots or earlier contents of memory.
 //
 // Masked scores become -inf and weigh 0, but 0 * NaN or 0 * inf of a V row
 // that only some of the CTA's rows may see would spoil the others.  So in
@@ -94,7 +97,10 @@ constexpr uint32_t kApmKvBytes = 16384;    // K or V block: 64 tokens x 128 dims
 constexpr uint32_t kApmKvHalf = 8192;
 constexpr uint32_t kApmOutBytes = 16384;   // 64 columns of a tile's output
 constexpr float kApmLazy = 16.f;   // growth of a row's maximum (base 2) that is left unscaled
-constexpr float kApmBound = 50.f; // largest reference (base 2) that may lie above the row's maximum
+// A capped score of at most this (base 2) may serve as reference in the place of
+// the row's maximum, which then lies at most twice as far below it: weights of
+// 2^-100 and sums of them are normal floats.
+constexpr float kApmBound = 50.f;
 constexpr int kApmMaxPos = 1 << 30;
 constexpr int kApmMinPiece = 8;   // key blocks of a piece at least, where an item is split
 constexpr size_t kApmQueueAt = 256, kApmFlagsAt = 1024;  // in the workspace's header
