@@ -91,9 +91,12 @@ def test_more_pairs_than_counters(torch_cuda):  # noqa: F811
     ref, ref_lse, tol, tol_lse = orc.paged_attention_mod(q.float().cpu().numpy().reshape(S, H, 128), c.pool, table, rows, H,
                                                          K, tpb)
     keep = [t for t, r in enumerate(rows) if r is not None and lens[t] > 0]
-    for _ in range(2):
-        out.fill_(9.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
         _lib.paged_attention_decode_mod(a)
+    for call in (lambda: _lib.paged_attention_decode_mod(a), graph.replay, graph.replay):
+        out.fill_(9.0)
+        call()
         assert _lib.read_status(ws) == (0, 0)
         got = out.float().cpu().numpy().reshape(S, H, 128)
         assert (np.abs(got - ref) <= tol)[keep].all()
