@@ -700,8 +700,13 @@ __global__ void __launch_bounds__(kApmThreads, 1)
           for (int i = 0; i < 8; ++i) {
             uint4 q = v[i * 128 + r];
             if ((not_finite2(q.x) | not_finite2(q.y) | not_finite2(q.z) | not_finite2(q.w)) != 0) {
-              *reinterpret_cast<volatile int*>(&tl->poison[k & 1]) = k + 1;
-              __threadfence_block();
+              // (slots that no row sees need not be added back: their scan would take 50
+              // times the call itself where a fresh cache holds NaN)
+              const int key = j0 + (((i * 128 + r) >> 3) & 63);
+              if (key >= at->lo_all && key < at->hi_all) {
+                *reinterpret_cast<volatile int*>(&tl->poison[k & 1]) = k + 1;
+                __threadfence_block();
+              }
               auto clean = [](uint32_t w) {
                 const uint32_t f = not_finite2(w);
                 return w & ((f & 0x8000u ? 0u : 0xFFFFu) | (f & 0x80000000u ? 0u : 0xFFFF0000u));

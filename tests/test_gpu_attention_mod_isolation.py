@@ -87,3 +87,32 @@ def test_prefill_one_row_live(torch_cuda):  # noqa: F811
     dead = [t for t in range(64) if t != 13]
     c.q_d[dead] = float("nan")
     assert same(outputs(c, a, torch), want)
+
+
+@pytest.mark.parametrize("q_lens,ctx,window", [([61], [0], 0), ([100] * 30, [0] * 30, 0), ([203, 90], [1001, 30], 300)])
+def test_unwritten_slots_cost_nothing(torch_cuda, q_lens, ctx, window):  # noqa: F811
+    """A fresh cache may hold NaN behind the last token; the same call on zeros there takes as long (a scan for values to
+    add back made it 50 times as long, the bound is 5)."""
+    torch = torch_cuda
+    c = Case(torch, ctx, q_lens=q_lens, n_heads=32, n_kv_heads=8, seed=75)
+    a = c.args(window=window)
+    unseen = torch.ones(c.blocks, c.tpb, dtype=torch.bool, device="cuda")
+    for s in range(c.S):
+        for j in range(c.total[s]):
+            unseen[c.table[s, j // 16], j % 16] = False
+    took = {}
+    for fill in (0.0, float("nan")):
+        c.pool_d[unseen] = fill
+        c.launch(a)
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        times = []
+        for _ in range(5):
+            start.record()
+            for _ in range(10):
+                c.launch(a)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        took[fill == 0.0] = min(times)
+    assert torch.isfinite(c.out).all()
+    assert took[False] < 5 * took[True], took
